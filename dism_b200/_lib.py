@@ -32,6 +32,12 @@ SIGNATURES = {
     'dism_profile_enable': (_I, [_I]),
     'dism_profile_count': (_I, []),
     'dism_profile_read': (_I, [_I, _c.c_char_p, _I, _c.POINTER(_c.c_float)]),
+    'dism_delta_saved': (_Z, [_I] * 8),
+    'dism_delta_forward': (_I, [_P] * 5 + [_I, _P, _P] + [_I] * 6 + [_c.c_float, _P, _P, _I, _P, _Z, _P]),
+    'dism_delta_backward_workspace': (_Z, [_I] * 6),
+    'dism_delta_backward': (_I, [_P] * 4 + [_I, _P] + [_I] * 6 + [_c.c_float, _P, _Z] + [_P] * 7 + [_Z, _P]),
+    'dism_delta_step': (_I, [_P] * 5 + [_I, _P, _P, _c.c_int64] + [_I] * 5 + [_c.c_float, _P, _P]),
+    'dism_dropout': (_I, [_I, _P, _P, _c.c_int64, _I, _P, _c.c_uint32, _P, _P]),
     'dism_longest_match': (_I, [_P, _I, _I, _P, _P, _P, _P, _Z, _P]),
 }
 

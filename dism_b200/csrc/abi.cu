@@ -2,7 +2,7 @@
 // The messages keep the key words the reference's checks use ("256-aligned", "CTA", "too short"),
 // so callers that match on them keep working.
 #include "../../include/dism_b200.h"
-#include "dism_common.cuh"
+#include "delta_common.cuh"
 
 #include <climits>
 #include <cstdarg>
@@ -93,7 +93,7 @@ int dism_profile_read(int index, char* name, int capacity, float* milliseconds) 
 }
 
 const char* dism_last_error(void) { return last_error; }
-int dism_abi_version(void) { return 9; }
+int dism_abi_version(void) { return 10; }
 
 int dism_route_word(const uint32_t* choice) {
     if (choice && !aligned(choice, 4)) return fail(DISM_EINVAL, "graph choice must be one aligned device int32");
@@ -298,6 +298,138 @@ int dism_longest_match(const int32_t* streams, int batch, int n, int32_t* end, i
         return fail(DISM_EINVAL, "workspace missing, too small or misaligned (see dism_longest_match_workspace)");
     return cuda_status(dism::launch_longest_match(streams, batch, n, end, length, next, workspace,
                                                   static_cast<cudaStream_t>(stream)), "longest_match");
+}
+
+// ---- gated delta rule ---------------------------------------------------------------------------------
+static int check_delta(int packed, int sequences, int n, int key_heads, int heads, int d, int dv) {
+    if (sequences <= 0 || n <= 0 || n > INT_MAX - 256 || key_heads <= 0 || heads <= 0) return fail(DISM_EINVAL, "positive dimensions required");
+    if (heads > 65535 || heads % key_heads) return fail(DISM_EINVAL, "value heads must be a multiple of the key heads and not exceed 65535");
+    if ((d != 32 && d != 64 && d != 128) || (dv != 32 && dv != 64 && dv != 128))
+        return fail(DISM_EUNSUPPORTED, "unsupported delta rule shape D=%d DV=%d (each in {32,64,128})", d, dv);
+    if (dism::DeltaLayout{packed ? reinterpret_cast<const int*>(4) : nullptr, sequences, n}.slots() > INT_MAX)
+        return fail(DISM_EINVAL, "too many chunks: sequences * n / 64 must fit 31 bits");
+    return DISM_OK;
+}
+
+namespace {
+constexpr size_t round_up(size_t bytes) { return (bytes + 255) / 256 * 256; }
+// The parts of `saved`, in the order in which they lie; those that `exact` or `backward` do not ask for have no bytes.
+size_t lay_out_delta(const dism::DeltaShape& shape, bool exact, bool backward, char* base, dism::DeltaSaved* saved) {
+    const size_t places = size_t(shape.layout.slots()) * shape.heads;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        char* part = base ? base + at : nullptr;
+        at += round_up(bytes);
+        return part;
+    };
+    using bf = __nv_bfloat16;
+    dism::DeltaSaved parts{};
+    parts.rows = reinterpret_cast<float*>(take(places * dism::ROW_VALUES * 4));
+    parts.t = reinterpret_cast<bf*>(take(places * dism::MATRIX * 2));
+    parts.p = reinterpret_cast<bf*>(take(places * dism::MATRIX * 2));
+    if (backward) {
+        parts.states = reinterpret_cast<bf*>(take(places * shape.d * shape.dv * 2));
+        parts.x = reinterpret_cast<bf*>(take(places * dism::CHUNK * shape.dv * 2));
+    }
+    if (exact) parts.t_rest = reinterpret_cast<bf*>(take(places * dism::MATRIX * 2));
+    if (saved) *saved = parts;
+    return at;
+}
+size_t delta_scratch(const dism::DeltaShape& shape, char* base, dism::DeltaGradients* x) {
+    const size_t places = size_t(shape.layout.slots()) * shape.heads;
+    const size_t states = round_up(places * shape.d * shape.dv * 2);
+    if (x) {
+        x->dstates = reinterpret_cast<__nv_bfloat16*>(base);
+        x->dbeta_parts = reinterpret_cast<float*>(base + states);
+    }
+    return states + round_up(places * dism::CHUNK * (shape.dv / 16) * 4);
+}
+dism::DeltaShape delta_shape(const int32_t* cu_seqlens, int sequences, int n, int key_heads, int heads, int d, int dv, int gates_bf16, float scale) {
+    return dism::DeltaShape{dism::DeltaLayout{cu_seqlens, sequences, n}, key_heads, heads, d, dv, gates_bf16 != 0, scale};
+}
+}  // namespace
+
+size_t dism_delta_saved(int packed, int sequences, int n, int heads, int d, int dv, int final_state, int backward) {
+    if (check_delta(packed, sequences, n, 1, heads, d, dv)) return 0;
+    const auto shape = delta_shape(packed ? reinterpret_cast<const int32_t*>(4) : nullptr, sequences, n, 1, heads, d, dv, 0, 1.f);
+    return lay_out_delta(shape, final_state != 0, backward != 0, nullptr, nullptr);
+}
+
+size_t dism_delta_backward_workspace(int packed, int sequences, int n, int heads, int d, int dv) {
+    if (check_delta(packed, sequences, n, 1, heads, d, dv)) return 0;
+    const auto shape = delta_shape(packed ? reinterpret_cast<const int32_t*>(4) : nullptr, sequences, n, 1, heads, d, dv, 0, 1.f);
+    return delta_scratch(shape, nullptr, nullptr);
+}
+
+int dism_delta_forward(const void* q, const void* k, const void* v, const void* g, const void* beta, int gates_bf16, const float* initial_state,
+                       const int32_t* cu_seqlens, int sequences, int n, int key_heads, int heads, int d, int dv, float scale, void* out,
+                       float* final_state, int backward, void* saved, size_t saved_bytes, void* stream) {
+    if (int status = check_delta(cu_seqlens != nullptr, sequences, n, key_heads, heads, d, dv)) return status;
+    if (!q || !k || !v || !g || !beta || !out) return fail(DISM_EINVAL, "null pointer");
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16)) return fail(DISM_EINVAL, "vector tensors must be 16-byte aligned");
+    if (!aligned(initial_state, 16) || !aligned(final_state, 16) || !aligned(g, gates_bf16 ? 2 : 4) || !aligned(beta, gates_bf16 ? 2 : 4) || !aligned(cu_seqlens, 4))
+        return fail(DISM_EINVAL, "states must be 16-byte aligned, gates and sequence starts to their size");
+    const auto shape = delta_shape(cu_seqlens, sequences, n, key_heads, heads, d, dv, gates_bf16, scale);
+    dism::DeltaSaved parts;
+    if (!saved || !aligned(saved, 256) || saved_bytes < lay_out_delta(shape, final_state != nullptr, backward != 0, static_cast<char*>(saved), &parts))
+        return fail(DISM_EINVAL, "workspace missing, too small or misaligned (see dism_delta_saved)");
+    using bf = __nv_bfloat16;
+    if (cudaError_t status = dism::launch_delta_prepare(shape, static_cast<const bf*>(q), static_cast<const bf*>(k), g, beta, parts, static_cast<cudaStream_t>(stream)))
+        return cuda_status(status, "delta_prepare");
+    return cuda_status(dism::launch_delta_chain(shape, static_cast<const bf*>(q), static_cast<const bf*>(k), static_cast<const bf*>(v), initial_state,
+                                                parts, static_cast<bf*>(out), final_state, static_cast<cudaStream_t>(stream)), "delta_chain");
+}
+
+int dism_delta_backward(const void* q, const void* k, const void* dout, const float* dfinal_state, int gates_bf16, const int32_t* cu_seqlens,
+                        int sequences, int n, int key_heads, int heads, int d, int dv, float scale, const void* saved, size_t saved_bytes,
+                        void* dq, void* dk, void* dv_out, void* dg, void* dbeta, float* dinitial_state, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+    if (int status = check_delta(cu_seqlens != nullptr, sequences, n, key_heads, heads, d, dv)) return status;
+    if (!q || !k || !dout || !dq || !dk || !dv_out || !dg || !dbeta) return fail(DISM_EINVAL, "null pointer");
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(dout, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv_out, 16))
+        return fail(DISM_EINVAL, "vector tensors must be 16-byte aligned");
+    if (!aligned(dfinal_state, 16) || !aligned(dinitial_state, 16) || !aligned(dg, gates_bf16 ? 2 : 4) || !aligned(dbeta, gates_bf16 ? 2 : 4) || !aligned(cu_seqlens, 4))
+        return fail(DISM_EINVAL, "states must be 16-byte aligned, gates and sequence starts to their size");
+    const auto shape = delta_shape(cu_seqlens, sequences, n, key_heads, heads, d, dv, gates_bf16, scale);
+    dism::DeltaSaved parts;
+    if (!saved || !aligned(saved, 256) || saved_bytes < lay_out_delta(shape, false, true, const_cast<char*>(static_cast<const char*>(saved)), &parts))
+        return fail(DISM_EINVAL, "saved buffer missing, too small or misaligned (see dism_delta_saved)");
+    using bf = __nv_bfloat16;
+    dism::DeltaGradients x{static_cast<const bf*>(q), static_cast<const bf*>(k), static_cast<const bf*>(dout), dfinal_state, nullptr, nullptr,
+                           static_cast<bf*>(dq), static_cast<bf*>(dk), static_cast<bf*>(dv_out), dg, dbeta, dinitial_state};
+    if (!workspace || !aligned(workspace, 256) || workspace_bytes < delta_scratch(shape, static_cast<char*>(workspace), &x))
+        return fail(DISM_EINVAL, "workspace missing, too small or misaligned (see dism_delta_backward_workspace)");
+    return cuda_status(dism::launch_delta_backward(shape, x, parts, static_cast<cudaStream_t>(stream)), "delta_backward");
+}
+
+int dism_delta_step(const void* q, const void* k, const void* v, const void* g, const void* beta, int gates_bf16, float* state,
+                    const int32_t* slots, int64_t pool, int batch, int key_heads, int heads, int d, int dv, float scale, void* out,
+                    void* stream) {
+    if (int status = check_delta(0, 1, 1, key_heads, heads, d, dv)) return status;
+    if (batch <= 0 || batch > 65535 || pool <= 0) return fail(DISM_EINVAL, "1..65535 rows and a positive number of states required");
+    if (!q || !k || !v || !g || !beta || !state || !out) return fail(DISM_EINVAL, "null pointer");
+    if (!slots && pool < batch) return fail(DISM_EINVAL, "without slots every row needs a state of its own");
+    if (!aligned(q, 2) || !aligned(k, 2) || !aligned(v, 8) || !aligned(out, 8) || !aligned(state, 16) || !aligned(g, gates_bf16 ? 2 : 4) ||
+        !aligned(beta, gates_bf16 ? 2 : 4) || !aligned(slots, 4))
+        return fail(DISM_EINVAL, "states must be 16-byte aligned, values 8-byte aligned");
+    using bf = __nv_bfloat16;
+    return cuda_status(dism::launch_delta_step(static_cast<const bf*>(q), static_cast<const bf*>(k), static_cast<const bf*>(v), g, beta,
+                                               gates_bf16 != 0, scale, state, slots, pool, batch, key_heads, heads, d, dv,
+                                               static_cast<bf*>(out), static_cast<cudaStream_t>(stream)), "delta_step");
+}
+
+int dism_dropout(int type, const void* x, const void* residual, int64_t count, int threshold, const int64_t* seed, uint32_t site, void* out,
+                 void* stream) {
+    if (type < 0 || type > 2) return fail(DISM_EUNSUPPORTED, "unsupported dropout type %d (0 float32, 1 float16, 2 bfloat16)", type);
+    if (count <= 0 || count > (int64_t(1) << 35)) return fail(DISM_EINVAL, "1 .. 2^35 elements required");
+    if (threshold < 0 || threshold > 65536) return fail(DISM_EINVAL, "the threshold must lie in 0 .. 65536");
+    if (!x || !seed || !out) return fail(DISM_EINVAL, "null pointer");
+    const size_t size = type ? 2 : 4;
+    if (!aligned(x, size) || !aligned(residual, size) || !aligned(out, size) || !aligned(seed, 8))
+        return fail(DISM_EINVAL, "tensors must be aligned to their element size");
+    const float scale = threshold < 65536 ? 65536.f / float(65536 - threshold) : 0.f;
+    return cuda_status(dism::launch_dropout(type, x, residual, count, unsigned(threshold), scale, seed, site, out,
+                                            static_cast<cudaStream_t>(stream)), "dropout");
 }
 
 }  // extern "C"

@@ -1,0 +1,173 @@
+// Shared parts of the gated delta rule kernels.
+//
+// The rule, per value head, with a state S [D, DV]:
+//     S_t = a_t S_{t-1} + k_t u_t^T,   u_t = b_t (v_t - a_t S_{t-1}^T k_t),   o_t = scale S_t^T q_t,   a_t = exp(g_t).
+// Over a chunk of 64 positions that starts from S0, with G the running sum of g inside the chunk, E_ts = exp(G_t - G_s),
+// L the strictly lower part of E * (K K^T) and T = (I + L diag(b))^-1:
+//     Y = V - e^G K S0,   X = T Y,   U = b X,   O = scale e^G Q S0 + P U,   P = scale tril(E * Q K^T),
+//     S1 = e^{G_63} S0 + K^T (e^{G_63 - G} U).
+// T depends on K, g and b alone, so one parallel kernel forms T and P of every chunk (delta_prepare.cu) and only products
+// with the state are left to the chain of chunks (delta_forward.cu).  T = I - (products of contractions), so for key
+// vectors of length one its entries stay within one: the inverse is well conditioned and survives a bf16 rounding.
+//
+// A fragment notation used throughout: mma.m16n8k16 keeps its 16 x 8 accumulator as (row lane/4 and lane/4 + 8, columns
+// 2 (lane%4) and +1); two neighbouring accumulators, rounded to bf16 and packed in pairs, are the 16 x 16 left operand of
+// the next product.  Everything that depends on the state is computed transposed ([dv, position] and [dv, d]), so a warp
+// owns 16 columns of the state for the whole sequence and the chain of products never leaves its registers.
+#pragma once
+#include "dism_common.cuh"
+
+namespace dism {
+
+constexpr int CHUNK = 64;
+constexpr int ROW_VALUES = 5 * CHUNK;      // per chunk and head: decay, beta, tail, and G as a pair of floats
+constexpr int MATRIX = CHUNK * CHUNK;      // elements of T and P of one chunk and head
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned smem_address(const void* p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void ldsm4(unsigned (&r)[4], unsigned address) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(unsigned (&r)[4], unsigned address) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
+}
+__device__ __forceinline__ void stsm4_trans(unsigned address, unsigned r0, unsigned r1, unsigned r2, unsigned r3) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(address), "r"(r0), "r"(r1), "r"(r2),
+                 "r"(r3) : "memory");
+}
+__device__ __forceinline__ unsigned pack2(float lo, float hi) {
+    __nv_bfloat162 pair = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<unsigned*>(&pair);
+}
+__device__ __forceinline__ float low_half(unsigned x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float high_half(unsigned x) { return __uint_as_float(x & 0xffff0000u); }
+// What the rounding to bf16 left out, as bf16 again: value and remainder carry 16 bits between them.
+__device__ __forceinline__ unsigned pack2_rest(float lo, float hi, unsigned rounded) {
+    return pack2(lo - low_half(rounded), hi - high_half(rounded));
+}
+// Two neighbouring accumulators (columns 16 j .. 16 j + 15) as the left operand of the next product.
+__device__ __forceinline__ void to_operand(unsigned (&a)[4], const float (&c0)[4], const float (&c1)[4]) {
+    a[0] = pack2(c0[0], c0[1]), a[1] = pack2(c0[2], c0[3]), a[2] = pack2(c1[0], c1[1]), a[3] = pack2(c1[2], c1[3]);
+}
+__device__ __forceinline__ void to_operand_rest(unsigned (&r)[4], const unsigned (&a)[4], const float (&c0)[4], const float (&c1)[4]) {
+    r[0] = pack2_rest(c0[0], c0[1], a[0]), r[1] = pack2_rest(c0[2], c0[3], a[1]);
+    r[2] = pack2_rest(c1[0], c1[1], a[2]), r[3] = pack2_rest(c1[2], c1[3], a[3]);
+}
+
+// Byte offsets a lane passes to ldmatrix / stmatrix for a 16 x 16 tile of a row-major matrix with `pitch` bytes a row.
+// rows_first: matrices in the order (rows 0-7, cols 0-7), (rows 8-15, cols 0-7), (rows 0-7, cols 8-15), (rows 8-15, cols 8-15);
+// cols_first: the two middle ones exchanged.
+__device__ __forceinline__ unsigned rows_first(int lane, int pitch) { return ((lane & 7) + (lane & 8)) * pitch + (lane >> 4) * 16; }
+__device__ __forceinline__ unsigned cols_first(int lane, int pitch) { return ((lane & 7) + ((lane >> 4) << 3)) * pitch + ((lane >> 3) & 1) * 16; }
+// The same for matrices stored as 8 x 8 blocks of 128 contiguous bytes, `width` blocks to a row of blocks (how the kernels
+// keep T, P and the states between each other: fragments leave and enter in whole lines and no access has a bank conflict).
+__device__ __forceinline__ unsigned rows_first_blocked(int lane, int width) { return (((lane >> 3) & 1) * width + (lane >> 4)) * 128 + (lane & 7) * 16; }
+__device__ __forceinline__ unsigned cols_first_blocked(int lane, int width) { return ((lane >> 4) * width + ((lane >> 3) & 1)) * 128 + (lane & 7) * 16; }
+
+// Where the sequences lie.  Fixed layout: `sequences` rows of n positions.  Packed: one row of n positions, document i at
+// [cu[i], cu[i+1]).  Every chunk has a slot of its own: in a pack, document i starts at slot cu[i] / 64 + i, which leaves
+// room for its last, partly filled chunk and needs no running sum over the documents.  Entries of cu are clamped to the
+// pack, so whatever they hold, every access stays inside the tensors.
+struct DeltaLayout {
+    const int* cu;
+    int sequences, n;
+    __host__ __device__ int chunks() const { return (n + CHUNK - 1) / CHUNK; }
+    __host__ __device__ int64_t slots() const { return cu ? int64_t(n / CHUNK) + sequences : int64_t(sequences) * chunks(); }
+    __device__ int start(int i) const { return min(max(__ldg(cu + i), 0), n); }
+    __device__ void span(int sequence, int64_t& row, int& length, int64_t& slot) const {
+        if (!cu) {
+            row = int64_t(sequence) * n, length = n, slot = int64_t(sequence) * chunks();
+            return;
+        }
+        const int begin = start(sequence);
+        row = begin, length = max(start(sequence + 1) - begin, 0), slot = begin / CHUNK + sequence;
+    }
+    // Row and number of positions of the chunk in a slot; zero positions when the slot is not used.
+    __device__ void chunk(int64_t slot, int64_t& row, int& count) const {
+        int64_t first;
+        int length, sequence;
+        if (!cu) {
+            sequence = int(slot / chunks());
+        } else {
+            int lo = 0, hi = sequences - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (start(mid) / CHUNK + mid <= slot) lo = mid;
+                else hi = mid - 1;
+            }
+            sequence = lo;
+        }
+        span(sequence, row, length, first);
+        const int64_t before = (slot - first) * CHUNK;
+        count = before < 0 ? 0 : int(min(int64_t(CHUNK), max(int64_t(length) - before, int64_t(0))));
+        row += max(before, int64_t(0));
+    }
+};
+
+struct DeltaShape {
+    DeltaLayout layout;
+    int key_heads, heads, d, dv;
+    bool gates_bf16;
+    float scale;
+};
+
+// What the kernels hand to one another, per slot and value head.  The backward needs all of it.
+struct DeltaSaved {
+    float* rows;               // [slots, H, ROW_VALUES]
+    __nv_bfloat16 *t, *t_rest; // [slots, H, MATRIX] blocked; t_rest only for an exact state
+    __nv_bfloat16* p;
+    __nv_bfloat16 *states, *x; // S0 [slots, H, DV, D] blocked and X [slots, H, CHUNK, DV]; only for a backward
+};
+
+__device__ __forceinline__ float gate(const void* gates, int64_t index, bool is_bf16) {
+    return is_bf16 ? bf2f(static_cast<const __nv_bfloat16*>(gates)[index]) : static_cast<const float*>(gates)[index];
+}
+
+// Copies `count` rows of `bytes` bytes (a multiple of 16) from a strided tensor into a padded tile of 64 rows; the rest is zeros.
+template <int BYTES, int THREADS>
+__device__ __forceinline__ void load_rows(unsigned tile, int pitch, const char* global, int64_t stride, int count, int thread) {
+    constexpr int PIECES = BYTES / 16;
+#pragma unroll
+    for (int i = thread; i < CHUNK * PIECES; i += THREADS) {
+        const int row = i / PIECES, piece = i % PIECES;
+        const bool inside = row < count;
+        const char* from = global + (inside ? row * stride : 0) + piece * 16;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tile + row * pitch + piece * 16), "l"(from),
+                     "r"(inside ? 16 : 0));
+    }
+}
+template <int BYTES, int THREADS>
+__device__ __forceinline__ void load_block(unsigned tile, const char* global, int thread) {
+#pragma unroll
+    for (int i = thread * 16; i < BYTES; i += THREADS * 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tile + i), "l"(global + i));
+}
+
+struct DeltaGradients {
+    const __nv_bfloat16 *q, *k, *dout;
+    const float* dfinal;  // gradient of the last states, or null
+    __nv_bfloat16* dstates;  // scratch: dS1 [slots, H, DV, D] blocked
+    float* dbeta_parts;      // scratch: [DV / 16, slots, H, CHUNK]
+    __nv_bfloat16 *dq, *dk, *dv;
+    void *dg, *dbeta;        // in the gates' type
+    float* dinitial;         // gradient of the first states, or null
+};
+
+cudaError_t launch_delta_prepare(const DeltaShape& shape, const __nv_bfloat16* q, const __nv_bfloat16* k, const void* g,
+                                 const void* beta, const DeltaSaved& saved, cudaStream_t stream);
+cudaError_t launch_delta_chain(const DeltaShape& shape, const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v,
+                               const float* initial, const DeltaSaved& saved, __nv_bfloat16* out, float* final_state,
+                               cudaStream_t stream);
+cudaError_t launch_delta_backward(const DeltaShape& shape, const DeltaGradients& gradients, const DeltaSaved& saved, cudaStream_t stream);
+cudaError_t launch_delta_step(const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v, const void* g, const void* beta,
+                              bool gates_bf16, float scale, float* state, const int* slots, int64_t pool, int batch, int key_heads,
+                              int heads, int d, int dv, __nv_bfloat16* out, cudaStream_t stream);
+
+}  // namespace dism

@@ -1,0 +1,263 @@
+// Chain of chunks of the gated delta rule, forward.
+//
+// A warp owns 16 columns of the state of one value head of one sequence and walks the chunks with the state, transposed, in
+// its accumulators.  Per chunk: S0 K^T and S0 Q^T (S0 rounded to bf16 straight from the accumulators), Y = V - e^G K S0,
+// X = T Y, U = b X, O = scale e^G Q S0 + P U, S1 = e^{G_63} S0 + K^T (e^{G_63 - G} U).  Warps share K, Q, T and P of the
+// chunk in shared memory, double-buffered with cp.async; nothing else passes between them.
+//
+// EXACT: the state is wanted at the end.  S0 in S0 K^T, Y, T and U are then kept as bf16 pairs (value and remainder, 16 bits),
+// which holds the state to a few 1e-6; without it a single bf16 is enough for outputs that are bf16 themselves.
+#include "delta_common.cuh"
+
+namespace dism {
+namespace {
+
+template <int D, int WARPS, bool EXACT>
+struct ForwardStage {
+    static constexpr int PITCH = 2 * D + 16, VALUE_PITCH = 32 * WARPS + 16;
+    static constexpr int K = 0, Q = K + CHUNK * PITCH, T = Q + CHUNK * PITCH, T_REST = T + 2 * MATRIX;
+    static constexpr int P = T_REST + (EXACT ? 2 * MATRIX : 0), V = P + 2 * MATRIX, ROWS = V + CHUNK * VALUE_PITCH;
+    static constexpr int BYTES = ROWS + 3 * CHUNK * 4;
+};
+
+template <int D, int WARPS, bool EXACT, bool SAVE>
+__global__ void __launch_bounds__(WARPS * 32) delta_chain_kernel(DeltaShape shape, const __nv_bfloat16* __restrict__ q,
+                                                                 const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v,
+                                                                 const float* __restrict__ initial, DeltaSaved saved,
+                                                                 __nv_bfloat16* __restrict__ out, float* __restrict__ final_state) {
+    using Stage = ForwardStage<D, WARPS, EXACT>;
+    constexpr int THREADS = WARPS * 32, TILES = CHUNK / 8;
+    extern __shared__ __align__(128) unsigned char shared[];
+    const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
+    const int head = blockIdx.y, sequence = blockIdx.x, dv = shape.dv;
+    const int key_head = head / (shape.heads / shape.key_heads), column = (blockIdx.z * WARPS + warp) * 16;
+    int64_t row, slot;
+    int length;
+    shape.layout.span(sequence, row, length, slot);
+    const int chunks = (length + CHUNK - 1) / CHUNK;
+    const unsigned base = smem_address(shared);
+
+    const int64_t key_stride = int64_t(shape.key_heads) * D * 2, value_stride = int64_t(shape.heads) * dv * 2;
+    auto load = [&](int c) {
+        const unsigned stage = base + (c & 1) * Stage::BYTES;
+        const int count = min(CHUNK, length - c * CHUNK);
+        const int64_t at = row + int64_t(c) * CHUNK, place = (slot + c) * shape.heads + head;
+        const int64_t key = (at * shape.key_heads + key_head) * D * 2;
+        load_rows<2 * D, THREADS>(stage + Stage::K, Stage::PITCH, reinterpret_cast<const char*>(k) + key, key_stride, count, thread);
+        load_rows<32 * WARPS, THREADS>(stage + Stage::V, Stage::VALUE_PITCH,
+                                       reinterpret_cast<const char*>(v) + ((at * shape.heads + head) * dv + blockIdx.z * WARPS * 16) * 2,
+                                       value_stride, count, thread);
+        load_block<3 * CHUNK * 4, THREADS>(stage + Stage::ROWS, reinterpret_cast<const char*>(saved.rows + place * ROW_VALUES), thread);
+        load_block<2 * MATRIX, THREADS>(stage + Stage::T, reinterpret_cast<const char*>(saved.t + place * MATRIX), thread);
+        if (EXACT) load_block<2 * MATRIX, THREADS>(stage + Stage::T_REST, reinterpret_cast<const char*>(saved.t_rest + place * MATRIX), thread);
+        load_rows<2 * D, THREADS>(stage + Stage::Q, Stage::PITCH, reinterpret_cast<const char*>(q) + key, key_stride, count, thread);
+        load_block<2 * MATRIX, THREADS>(stage + Stage::P, reinterpret_cast<const char*>(saved.p + place * MATRIX), thread);
+        cp_async_commit();
+    };
+
+    float s[D / 8][4];  // the state, transposed: 16 columns of S by D
+    const int64_t state_at = (int64_t(sequence) * shape.heads + head) * D * dv + column + (lane >> 2);
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            s[n][e] = initial ? __ldg(initial + state_at + int64_t(8 * n + 2 * (lane & 3) + (e & 1)) * dv + (e >> 1) * 8) : 0.f;
+    if (chunks > 0) load(0);
+    for (int c = 0; c < chunks; ++c) {
+        cp_async_wait<0>();
+        __syncthreads();  // chunk c is in, and every warp has left chunk c - 1
+        if (c + 1 < chunks) load(c + 1);
+        const unsigned stage = base + (c & 1) * Stage::BYTES;
+        const float* rows = reinterpret_cast<const float*>(shared + (c & 1) * Stage::BYTES + Stage::ROWS);
+        const int64_t place = (slot + c) * shape.heads + head;
+
+        float ks[TILES][4], qs[TILES][4];
+#pragma unroll
+        for (int n = 0; n < TILES; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ks[n][e] = qs[n][e] = 0.f;
+        const unsigned keys = stage + Stage::K + cols_first(lane, Stage::PITCH), queries = keys + Stage::Q - Stage::K;
+#pragma unroll
+        for (int kb = 0; kb < D / 16; ++kb) {
+            unsigned a[4], rest[4];
+            to_operand(a, s[2 * kb], s[2 * kb + 1]);
+            if (EXACT) to_operand_rest(rest, a, s[2 * kb], s[2 * kb + 1]);
+            if (SAVE) {
+                unsigned* to = reinterpret_cast<unsigned*>(saved.states + place * dv * D) + (int64_t(column / 8) * (D / 8) + 2 * kb) * 32 + lane;
+                to[0] = a[0], to[D / 8 * 32] = a[1], to[32] = a[2], to[D / 8 * 32 + 32] = a[3];
+            }
+#pragma unroll
+            for (int np = 0; np < TILES / 2; ++np) {
+                unsigned b[4];
+                ldsm4(b, keys + np * 16 * Stage::PITCH + kb * 32);
+                mma16816(ks[2 * np], a, b[0], b[1]);
+                mma16816(ks[2 * np + 1], a, b[2], b[3]);
+                if (EXACT) {
+                    mma16816(ks[2 * np], rest, b[0], b[1]);
+                    mma16816(ks[2 * np + 1], rest, b[2], b[3]);
+                }
+                ldsm4(b, queries + np * 16 * Stage::PITCH + kb * 32);
+                mma16816(qs[2 * np], a, b[0], b[1]);
+                mma16816(qs[2 * np + 1], a, b[2], b[3]);
+            }
+        }
+        // Y, as the left operand of X = T Y
+        const unsigned values = stage + Stage::V + warp * 32 + cols_first(lane, Stage::VALUE_PITCH);
+        unsigned y[TILES / 2][4], y_rest[EXACT ? TILES / 2 : 1][4];
+#pragma unroll
+        for (int np = 0; np < TILES / 2; ++np) {
+            unsigned vv[4];
+            ldsm4_trans(vv, values + np * 16 * Stage::VALUE_PITCH);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float(&tile)[4] = ks[2 * np + h];
+                const float2 decay = *reinterpret_cast<const float2*>(rows + 16 * np + 8 * h + 2 * (lane & 3));
+                tile[0] = low_half(vv[2 * h]) - decay.x * tile[0], tile[1] = high_half(vv[2 * h]) - decay.y * tile[1];
+                tile[2] = low_half(vv[2 * h + 1]) - decay.x * tile[2], tile[3] = high_half(vv[2 * h + 1]) - decay.y * tile[3];
+                const float sx = shape.scale * decay.x, sy = shape.scale * decay.y;
+                float(&o)[4] = qs[2 * np + h];
+                o[0] *= sx, o[1] *= sy, o[2] *= sx, o[3] *= sy;
+            }
+            to_operand(y[np], ks[2 * np], ks[2 * np + 1]);
+            if (EXACT) to_operand_rest(y_rest[np], y[np], ks[2 * np], ks[2 * np + 1]);
+        }
+        float(&x)[TILES][4] = ks;
+#pragma unroll
+        for (int n = 0; n < TILES; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[n][e] = 0.f;
+        const unsigned inverse = stage + Stage::T + cols_first_blocked(lane, TILES), inside = inverse + Stage::P - Stage::T;
+#pragma unroll
+        for (int np = 0; np < TILES / 2; ++np)
+#pragma unroll
+            for (int kb = 0; kb <= np; ++kb) {
+                unsigned b[4];
+                ldsm4(b, inverse + (np * 2 * TILES + kb * 2) * 128);
+                mma16816(x[2 * np], y[kb], b[0], b[1]);
+                mma16816(x[2 * np + 1], y[kb], b[2], b[3]);
+                if (EXACT) {
+                    mma16816(x[2 * np], y_rest[kb], b[0], b[1]);
+                    mma16816(x[2 * np + 1], y_rest[kb], b[2], b[3]);
+                    ldsm4(b, inverse + Stage::T_REST - Stage::T + (np * 2 * TILES + kb * 2) * 128);
+                    mma16816(x[2 * np], y[kb], b[0], b[1]);
+                    mma16816(x[2 * np + 1], y[kb], b[2], b[3]);
+                }
+            }
+        const int count = min(CHUNK, length - c * CHUNK);
+        // the warp's 16 columns of the value tile are its own: X and O leave through them in rows of 32 bytes
+        auto leave = [&](const float(&tiles)[TILES][4], char* to, int64_t stride, int rows_out) {
+            __syncwarp();
+#pragma unroll
+            for (int np = 0; np < TILES / 2; ++np) {
+                const float(&t0)[4] = tiles[2 * np], (&t1)[4] = tiles[2 * np + 1];
+                stsm4_trans(values + np * 16 * Stage::VALUE_PITCH, pack2(t0[0], t0[1]), pack2(t0[2], t0[3]), pack2(t1[0], t1[1]), pack2(t1[2], t1[3]));
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < CHUNK * 2 / 32; ++i) {
+                const int t = i * 16 + (lane >> 1);
+                const uint4 piece = *reinterpret_cast<const uint4*>(shared + (c & 1) * Stage::BYTES + Stage::V + t * Stage::VALUE_PITCH + warp * 32 + (lane & 1) * 16);
+                if (t < rows_out) *reinterpret_cast<uint4*>(to + t * stride + (lane & 1) * 16) = piece;
+            }
+        };
+        if (SAVE) leave(x, reinterpret_cast<char*>(saved.x + place * CHUNK * dv + column), int64_t(dv) * 2, CHUNK);
+        // U, as left operand of P U; then with the decay to the chunk's end, of the state's update
+        unsigned u[TILES / 2][4], u_rest[EXACT ? TILES / 2 : 1][4];
+#pragma unroll
+        for (int np = 0; np < TILES / 2; ++np) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float2 b = *reinterpret_cast<const float2*>(rows + CHUNK + 16 * np + 8 * h + 2 * (lane & 3));
+                float(&tile)[4] = x[2 * np + h];
+                tile[0] *= b.x, tile[1] *= b.y, tile[2] *= b.x, tile[3] *= b.y;
+            }
+            to_operand(u[np], x[2 * np], x[2 * np + 1]);
+        }
+#pragma unroll
+        for (int np = 0; np < TILES / 2; ++np)
+#pragma unroll
+            for (int kb = 0; kb <= np; ++kb) {
+                unsigned b[4];
+                ldsm4(b, inside + (np * 2 * TILES + kb * 2) * 128);
+                mma16816(qs[2 * np], u[kb], b[0], b[1]);
+                mma16816(qs[2 * np + 1], u[kb], b[2], b[3]);
+            }
+        leave(qs, reinterpret_cast<char*>(out + ((row + int64_t(c) * CHUNK) * shape.heads + head) * dv + column), value_stride, count);
+        const float kept = rows[CHUNK - 1];
+#pragma unroll
+        for (int np = 0; np < TILES / 2; ++np) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float2 tail = *reinterpret_cast<const float2*>(rows + 2 * CHUNK + 16 * np + 8 * h + 2 * (lane & 3));
+                float(&tile)[4] = x[2 * np + h];
+                tile[0] *= tail.x, tile[1] *= tail.y, tile[2] *= tail.x, tile[3] *= tail.y;
+            }
+            to_operand(u[np], x[2 * np], x[2 * np + 1]);
+            if (EXACT) to_operand_rest(u_rest[np], u[np], x[2 * np], x[2 * np + 1]);
+        }
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] *= kept;
+        const unsigned keys_trans = stage + Stage::K + rows_first(lane, Stage::PITCH);
+#pragma unroll
+        for (int kb = 0; kb < TILES / 2; ++kb)
+#pragma unroll
+            for (int np = 0; np < D / 16; ++np) {
+                unsigned b[4];
+                ldsm4_trans(b, keys_trans + kb * 16 * Stage::PITCH + np * 32);
+                mma16816(s[2 * np], u[kb], b[0], b[1]);
+                mma16816(s[2 * np + 1], u[kb], b[2], b[3]);
+                if (EXACT) {
+                    mma16816(s[2 * np], u_rest[kb], b[0], b[1]);
+                    mma16816(s[2 * np + 1], u_rest[kb], b[2], b[3]);
+                }
+            }
+    }
+    if (final_state) {
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                final_state[state_at + int64_t(8 * n + 2 * (lane & 3) + (e & 1)) * dv + (e >> 1) * 8] = s[n][e];
+    }
+}
+
+template <int D, int WARPS, bool EXACT, bool SAVE>
+cudaError_t launch(const DeltaShape& shape, const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v,
+                   const float* initial, const DeltaSaved& saved, __nv_bfloat16* out, float* final_state, cudaStream_t stream) {
+    constexpr int BYTES = 2 * ForwardStage<D, WARPS, EXACT>::BYTES;
+    auto* kernel = delta_chain_kernel<D, WARPS, EXACT, SAVE>;
+    if (cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES)) return status;
+    KernelTimer timer("delta_chain", stream);
+    kernel<<<dim3(shape.layout.sequences, shape.heads, shape.dv / (16 * WARPS)), WARPS * 32, BYTES, stream>>>(shape, q, k, v, initial, saved, out, final_state);
+    return cudaGetLastError();
+}
+
+template <int D, int WARPS>
+cudaError_t choose(const DeltaShape& shape, const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v,
+                   const float* initial, const DeltaSaved& saved, __nv_bfloat16* out, float* final_state, cudaStream_t stream) {
+    const bool exact = saved.t_rest != nullptr, save = saved.states != nullptr;
+    if (exact && save) return launch<D, WARPS, true, true>(shape, q, k, v, initial, saved, out, final_state, stream);
+    if (exact) return launch<D, WARPS, true, false>(shape, q, k, v, initial, saved, out, final_state, stream);
+    if (save) return launch<D, WARPS, false, true>(shape, q, k, v, initial, saved, out, final_state, stream);
+    return launch<D, WARPS, false, false>(shape, q, k, v, initial, saved, out, final_state, stream);
+}
+
+template <int D>
+cudaError_t by_width(const DeltaShape& shape, const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v,
+                     const float* initial, const DeltaSaved& saved, __nv_bfloat16* out, float* final_state, cudaStream_t stream) {
+    if (shape.dv % 64 == 0) return choose<D, 4>(shape, q, k, v, initial, saved, out, final_state, stream);
+    return choose<D, 2>(shape, q, k, v, initial, saved, out, final_state, stream);
+}
+}  // namespace
+
+cudaError_t launch_delta_chain(const DeltaShape& shape, const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v,
+                               const float* initial, const DeltaSaved& saved, __nv_bfloat16* out, float* final_state,
+                               cudaStream_t stream) {
+    if (shape.d == 32) return by_width<32>(shape, q, k, v, initial, saved, out, final_state, stream);
+    if (shape.d == 64) return by_width<64>(shape, q, k, v, initial, saved, out, final_state, stream);
+    return by_width<128>(shape, q, k, v, initial, saved, out, final_state, stream);
+}
+
+}  // namespace dism

@@ -206,5 +206,7 @@ cudaError_t launch_hard_backward(HardShape shape, const __nv_bfloat16* sq, const
                                  const float* lut, int lut_stride, const float* lse2, int ctas, float* dsq,
                                  __nv_bfloat16* dsk, __nv_bfloat16* dv, float* dtau, void* workspace, const void* readout_workspace,
                                  cudaStream_t stream);
+cudaError_t launch_dropout(int type, const void* x, const void* residual, int64_t count, unsigned threshold, float scale,
+                           const int64_t* seed, unsigned site, void* out, cudaStream_t stream);
 
 }  // namespace dism

@@ -13,6 +13,9 @@ the soft path (`core_forward`, `core_backward`) is not
 built and raises NotImplementedError.  The `choice` device word of the reference's CUDA-graph
 router (one CUDA int32; 0 runs the hard path, anything else makes its kernels return at once) is
 handed to the library for the calls of the operator it was given to.
+
+Beyond the reference's module: labels, labels_pair, longest_match, the gated delta rule (delta_forward, delta_backward,
+delta_step) and dropout.
 """
 import contextlib
 
@@ -467,6 +470,171 @@ def longest_match(streams):
         _lib.check(_abi.dism_longest_match(streams.data_ptr(), b, n, end.data_ptr(), length.data_ptr(),
                                            nxt.data_ptr(), workspace.data_ptr(), size, _stream(streams)))
     return end, length, nxt
+
+
+# ---- gated delta rule ------------------------------------------------------------------------------
+# The reference's hybrid layers (dism_v3/python/flash_dism/hybrid_gdn.py, pure_gdn.py) take this mixer from an outside
+# package; here it is part of the library, in the layouts of the other operators.
+def _delta_operands(q, k, v, g, beta, tail):
+    """Checks q, k [*,HK,D], v [*,H,DV], g and beta [*,H]; returns (HK, H, D, DV, gates are bf16)."""
+    _check(v, torch.bfloat16, None, 'v')
+    if v.dim() != tail + 2:
+        _fail('v must be [B,N,H,DV]' if tail == 2 else 'v must be [B,H,DV]')
+    _check(q, torch.bfloat16, None, 'q')
+    if q.dim() != v.dim() or q.shape[:tail] != v.shape[:tail] or q.device != v.device:
+        _fail('q: invalid device, dtype, shape or stride')
+    _check(k, torch.bfloat16, q.shape, 'k')
+    if not torch.is_tensor(g) or g.dtype not in (torch.float32, torch.bfloat16):
+        _fail('g must be float32 or bfloat16')
+    _check(g, g.dtype, v.shape[:-1], 'g')
+    _check(beta, g.dtype, v.shape[:-1], 'beta')
+    if any(x.device != v.device for x in (k, g, beta)):
+        _fail('operands on different devices')
+    key_heads, d, heads, dv = q.size(-2), q.size(-1), v.size(-2), v.size(-1)
+    if heads <= 0 or key_heads <= 0 or heads % key_heads:
+        _fail('value heads must be a multiple of the key heads')
+    if d not in (32, 64, 128) or dv not in (32, 64, 128):
+        _fail(f'unsupported delta rule shape D={d} DV={dv} (each in {{32,64,128}})')
+    return key_heads, heads, d, dv, g.dtype == torch.bfloat16
+
+
+def _delta_sequences(v, cu_seqlens):
+    """Number of sequences and the device pointer of their starts (0 = the rows of the batch)."""
+    if cu_seqlens is None:
+        return v.size(0), 0
+    if not (torch.is_tensor(cu_seqlens) and cu_seqlens.device == v.device and cu_seqlens.dtype == torch.int32
+            and cu_seqlens.dim() == 1 and cu_seqlens.numel() > 1 and cu_seqlens.is_contiguous()):
+        _fail('cu_seqlens must be contiguous int32 [sequences+1] on the operand device')
+    if v.size(0) != 1:
+        _fail('a pack is one batch row')
+    return cu_seqlens.numel() - 1, cu_seqlens.data_ptr()
+
+
+def _delta_state(state, sequences, heads, d, dv, device, name):
+    if state is None:
+        return None
+    if not torch.is_tensor(state) or state.device != device:
+        _fail(f'{name}: invalid device, dtype, shape or stride')
+    _check(state, torch.float32, (sequences, heads, d, dv), name)
+    return state.data_ptr()
+
+
+def delta_forward(x, scale, initial_state=None, final_state=False, cu_seqlens=None, covered=True, backward=False):
+    """x = (q, k bf16 [B,N,HK,D], v bf16 [B,N,H,DV], g, beta float or bf16 [B,N,H]) -> (out bf16 [B,N,H,DV], final state FP32
+    [sequences,H,D,DV] or None, saved buffer).  `covered`: the sequences are known to cover every row; otherwise rows of none are zeros.
+    With backward=True the saved buffer is what delta_backward needs; otherwise it is dead."""
+    if len(x) != 5:
+        _fail('expected q,k,v,g,beta')
+    q, k, v, g, beta = x
+    key_heads, heads, d, dv, gates_bf16 = _delta_operands(q, k, v, g, beta, 2)
+    sequences, starts = _delta_sequences(v, cu_seqlens)
+    initial = _delta_state(initial_state, sequences, heads, d, dv, v.device, 'initial state')
+    n = v.size(1)
+    with torch.cuda.device(v.device):
+        out = (torch.empty_like if covered else torch.zeros_like)(v)
+        final = torch.empty((sequences, heads, d, dv), dtype=torch.float32, device=v.device) if final_state else None
+        if n == 0 or sequences == 0:
+            if final is not None:
+                final.zero_() if initial_state is None else final.copy_(initial_state)
+            return out, final, None
+        size = _abi.dism_delta_saved(starts != 0, sequences, n, heads, d, dv, bool(final_state), bool(backward))
+        saved = torch.empty((size,), dtype=torch.uint8, device=v.device)
+        _lib.check(_abi.dism_delta_forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), gates_bf16,
+                                           initial, starts, sequences, n, key_heads, heads, d, dv, float(scale), out.data_ptr(),
+                                           final.data_ptr() if final_state else None, bool(backward), saved.data_ptr(), size,
+                                           _stream(v)))
+    return out, final, saved if backward else None
+
+
+def delta_backward(q, k, dout, scale, saved, gate_dtype, dfinal_state=None, initial_gradient=False, cu_seqlens=None, covered=True):
+    """Gradients of delta_forward(..., backward=True): [dq, dk bf16, dv bf16, dg, dbeta in gate_dtype, d(initial state) FP32 or None]."""
+    _check(q, torch.bfloat16, None, 'q')
+    _check(k, torch.bfloat16, q.shape, 'k')
+    _check(dout, torch.bfloat16, None, 'dO')
+    if dout.dim() != 4 or q.dim() != 4 or q.shape[:2] != dout.shape[:2] or k.device != q.device or dout.device != q.device:
+        _fail('dO: invalid device, dtype, shape or stride')
+    if gate_dtype not in (torch.float32, torch.bfloat16):
+        _fail('g must be float32 or bfloat16')
+    b, n, key_heads, d = q.shape
+    heads, dv = dout.shape[2:]
+    sequences, starts = _delta_sequences(dout, cu_seqlens)
+    dfinal = _delta_state(dfinal_state, sequences, heads, d, dv, q.device, 'final state gradient')
+    with torch.cuda.device(q.device):
+        fresh = torch.empty if covered else torch.zeros
+        dq, dk = (fresh(q.shape, dtype=q.dtype, device=q.device) for _ in range(2))
+        dvalue = fresh(dout.shape, dtype=dout.dtype, device=q.device)
+        dg, dbeta = (fresh((b, n, heads), dtype=gate_dtype, device=q.device) for _ in range(2))
+        dinitial = torch.empty((sequences, heads, d, dv), dtype=torch.float32, device=q.device) if initial_gradient else None
+        if n == 0 or sequences == 0:
+            if dinitial is not None:
+                dinitial.zero_() if dfinal_state is None else dinitial.copy_(dfinal_state)
+            return [dq, dk, dvalue, dg, dbeta, dinitial]
+        if not (torch.is_tensor(saved) and saved.device == q.device and saved.dtype == torch.uint8 and saved.is_contiguous()):
+            _fail('saved buffer: invalid device, dtype, shape or stride')
+        size = _abi.dism_delta_backward_workspace(starts != 0, sequences, n, heads, d, dv)
+        workspace = torch.empty((size,), dtype=torch.uint8, device=q.device)
+        _lib.check(_abi.dism_delta_backward(q.data_ptr(), k.data_ptr(), dout.data_ptr(), dfinal, gate_dtype == torch.bfloat16, starts,
+                                            sequences, n, key_heads, heads, d, dv, float(scale), saved.data_ptr(), saved.numel(),
+                                            dq.data_ptr(), dk.data_ptr(), dvalue.data_ptr(), dg.data_ptr(), dbeta.data_ptr(),
+                                            dinitial.data_ptr() if initial_gradient else None, workspace.data_ptr(), size, _stream(q)))
+    return [dq, dk, dvalue, dg, dbeta, dinitial]
+
+
+def delta_step(x, scale, state, slots=None):
+    """One token per row: x = (q, k bf16 [B,HK,D], v bf16 [B,H,DV], g, beta [B,H]), state FP32 [pool,H,D,DV], updated in place;
+    slots int32 [B] names each row's state (outside the pool: no sequence, zero output).  Returns bf16 [B,H,DV]."""
+    if len(x) != 5:
+        _fail('expected q,k,v,g,beta')
+    q, k, v, g, beta = x
+    key_heads, heads, d, dv, gates_bf16 = _delta_operands(q, k, v, g, beta, 1)
+    if not torch.is_tensor(state) or state.dim() != 4 or state.device != v.device:
+        _fail('state must be FP32 [pool,H,D,DV] on the operand device')
+    _delta_state(state, state.size(0), heads, d, dv, v.device, 'state')
+    batch = v.size(0)
+    if slots is None:
+        if state.size(0) != batch:
+            _fail('without slots every row needs a state of its own')
+    elif not (torch.is_tensor(slots) and slots.device == v.device and slots.dtype == torch.int32 and tuple(slots.shape) == (batch,)
+              and slots.is_contiguous()):
+        _fail('slots must be contiguous int32 [B] on the operand device')
+    with torch.cuda.device(v.device):
+        out = torch.empty_like(v)
+        if batch and state.size(0):
+            _lib.check(_abi.dism_delta_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), gates_bf16,
+                                            state.data_ptr(), None if slots is None else slots.data_ptr(), state.size(0), batch,
+                                            key_heads, heads, d, dv, float(scale), out.data_ptr(), _stream(v)))
+        elif batch:
+            out.zero_()
+    return out
+
+
+# ---- dropout ---------------------------------------------------------------------------------------
+_dropout_types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def dropout(x, residual, threshold, seed, site=0):
+    """residual + x * keep * 65536 / (65536 - threshold) with keep = (16-bit Philox number >= threshold); residual may be None.
+    seed is CUDA int64 [2]: (key, offset), read when the kernel runs."""
+    if not torch.is_tensor(x) or x.dtype not in _dropout_types:
+        _fail('x must be float32, float16 or bfloat16')
+    _check(x, x.dtype, None, 'x')
+    if residual is not None:
+        _check(residual, x.dtype, x.shape, 'residual')
+        if residual.device != x.device:
+            _fail('residual on another device')
+    if not (torch.is_tensor(seed) and seed.device == x.device and seed.dtype == torch.int64 and tuple(seed.shape) == (2,)
+            and seed.is_contiguous()):
+        _fail('seed must be contiguous CUDA int64 [2] on the device of x')
+    if not 0 <= threshold <= 65536:
+        _fail('the threshold must lie in 0 .. 65536')
+    if not 0 <= site < 1 << 32:
+        _fail('site must fit 32 bits')
+    with torch.cuda.device(x.device):
+        out = torch.empty_like(x)
+        if x.numel():
+            _lib.check(_abi.dism_dropout(_dropout_types[x.dtype], x.data_ptr(), None if residual is None else residual.data_ptr(),
+                                         x.numel(), int(threshold), seed.data_ptr(), int(site), out.data_ptr(), _stream(x)))
+    return out
 
 
 def core_forward(*args, **kwargs):

@@ -1,0 +1,109 @@
+"""Gated delta rule: the recurrent mixer beside DISM layers in a hybrid model, over whole sequences and one token at a time.
+
+The reference's hybrid layers call such an operator of an outside package (dism_v3/python/flash_dism/hybrid_gdn.py,
+pure_gdn.py); here it is part of the library.  Per value head, with a state S [D,DV]:
+
+    S_t = exp(g_t) S_{t-1} + k_t u_t^T,   u_t = beta_t (v_t - exp(g_t) S_{t-1}^T k_t),   o_t = scale S_t^T q_t
+"""
+import torch
+import cu_flash_dism as cu
+
+
+def _ready(t):
+    """Contiguous and 16-byte aligned, as the library wants its tensors; a copy only where it is needed."""
+    t = t.detach().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class _GatedDelta(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, initial_state, scale, final_state, starts, covered, needed):
+        gates = g.dtype if g.dtype == beta.dtype and g.dtype in (torch.float32, torch.bfloat16) else torch.float32
+        initial = None if initial_state is None else _ready(initial_state)
+        ready_q, ready_k = _ready(q), _ready(k)
+        out, final, saved = cu.delta_forward((ready_q, ready_k, _ready(v), _ready(g.to(gates)), _ready(beta.to(gates))), scale,
+                                             initial, final_state, starts, covered, needed)
+        if needed:
+            ctx.save_for_backward(ready_q, ready_k, saved, starts)
+            ctx.types, ctx.gates, ctx.scale, ctx.covered = (g.dtype, beta.dtype), gates, scale, covered
+            ctx.set_materialize_grads(False)
+            ctx.shape = v.shape
+        return out, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dfinal):
+        q, k, saved, starts = ctx.saved_tensors
+        dout = torch.zeros(ctx.shape, dtype=torch.bfloat16, device=q.device) if dout is None else _ready(dout)
+        dfinal = None if dfinal is None else _ready(dfinal)
+        dq, dk, dv, dg, dbeta, dinitial = cu.delta_backward(q, k, dout, ctx.scale, saved, ctx.gates, dfinal, ctx.needs_input_grad[5],
+                                                            starts, ctx.covered)
+        return dq, dk, dv, dg.to(ctx.types[0]), dbeta.to(ctx.types[1]), dinitial, None, None, None, None, None
+
+
+_starts = {}
+
+
+def _host_starts(starts, device):
+    """Uploads document starts once per distinct pack and device."""
+    key = (tuple(starts), str(device))
+    cached = _starts.get(key)
+    if cached is None:
+        if len(_starts) >= 32:
+            _starts.pop(next(iter(_starts)))
+        cached = _starts[key] = torch.tensor(starts, dtype=torch.int32).to(device)
+    return cached
+
+
+def _documents(v, cu_seqlens, layout):
+    """Device starts of the documents and whether they are known to cover every row."""
+    if cu_seqlens is not None and layout is not None:
+        raise ValueError('provide either layout or cu_seqlens, not both')
+    if layout is not None:
+        starts = [0]
+        for length in layout.lengths:
+            starts.append(starts[-1] + length)
+        if v.dim() != 4 or starts[-1] != v.size(1):
+            raise ValueError('layout and operands differ in length')
+        return _host_starts(starts, v.device), True
+    if cu_seqlens is None:
+        return None, True
+    if not (torch.is_tensor(cu_seqlens) and cu_seqlens.dim() == 1 and cu_seqlens.dtype == torch.int32 and cu_seqlens.numel() > 1):
+        raise RuntimeError('cu_seqlens must be int32 [sequences+1]')
+    if cu_seqlens.device.type == 'cpu':
+        starts = cu_seqlens.tolist()
+        if v.dim() != 4 or starts[0] != 0 or starts[-1] != v.size(1) or any(a > b for a, b in zip(starts, starts[1:])):
+            raise RuntimeError('invalid cu_seqlens: starts at 0, ascending, ends at the number of positions')
+        return _host_starts(starts, v.device), True
+    return cu_seqlens.contiguous(), False
+
+
+def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, output_final_state=False, cu_seqlens=None, layout=None):
+    """BF16 q, k [B,N,HK,D] and v [B,N,H,DV], log decay g and write strength beta [B,N,H] (float32 or bfloat16) -> BF16
+    [B,N,H,DV]; with output_final_state=True also the FP32 state [sequences,H,D,DV] after each sequence's last position.
+
+    H is a multiple of HK (value head h reads key head h // (H // HK)), D and DV in {32,64,128}, N any length.  Keys are meant to
+    have length one at most; the caller normalises.  scale defaults to D ** -0.5.  g = -inf clears the state.  A pack is one
+    batch row with either `layout` (a VarlenLayout) or `cu_seqlens`, int32 [documents+1]; documents may have any length, zero
+    included.  On the CPU cu_seqlens is validated; on the GPU it is read by the kernels only (so a captured graph can follow new
+    lengths), must ascend, and rows outside [cu_seqlens[0], cu_seqlens[-1]) come out as zeros.  initial_state is FP32
+    [sequences,H,D,DV].  All operands and the initial state are differentiable; gates receive gradients in their own type, with
+    the relative accuracy of the bf16 operands.  Keeping the states for a backward takes 2 D DV / 64 + 2 DV + 276 bytes per position
+    and head."""
+    starts, covered = _documents(v, cu_seqlens, layout)
+    needed = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
+    out, final = _GatedDelta.apply(q, k, v, g, beta, initial_state, q.size(-1) ** -.5 if scale is None else float(scale),
+                                   bool(output_final_state), starts, covered, needed)
+    return (out, final) if output_final_state else out
+
+
+@torch.no_grad()
+def gated_delta_step(q, k, v, g, beta, state, *, scale=None, slots=None):
+    """One token for every row of a decoding batch: q, k BF16 [B,HK,D], v BF16 [B,H,DV], g and beta [B,H] -> BF16 [B,H,DV].
+
+    `state` is FP32 [pool,H,D,DV], contiguous, and is updated in place.  `slots`, int32 [B] on the GPU, names the state of each
+    row (default: state i for row i); a slot outside the pool marks a padding row, whose output is zero, and rows that name
+    one slot are consecutive tokens of that sequence, in row order.  Everything is computed in 32 bits; not differentiable."""
+    gates = g.dtype if g.dtype == beta.dtype and g.dtype in (torch.float32, torch.bfloat16) else torch.float32
+    return cu.delta_step((_ready(q), _ready(k), _ready(v), _ready(g.to(gates)), _ready(beta.to(gates))),
+                         q.size(-1) ** -.5 if scale is None else float(scale), state, slots)

@@ -161,6 +161,48 @@ size_t dism_longest_match_workspace(int batch, int n);
 int dism_longest_match(const int32_t *streams, int batch, int n, int32_t *end, int32_t *length,
                        int32_t *next, void *workspace, size_t workspace_bytes, void *stream);
 
+/* Gated delta rule, the other sequence mixer of a hybrid model (the reference's hybrid layers:
+ * dism_v3/python/flash_dism/hybrid_gdn.py, pure_gdn.py).  Per value head, with a state S [D,DV] in FP32:
+ *   S_t = exp(g_t) S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - exp(g_t) S_{t-1}^T k_t),  o_t = scale S_t^T q_t.
+ * q, k bf16 [B,N,HK,D]; v, out bf16 [B,N,H,DV], H a multiple of HK (value head h reads key head h / (H/HK));
+ * g (natural-log decay; minus infinity clears the state) and beta [B,N,H], float or (gates_bf16) bf16; D, DV in {32,64,128};
+ * any N.  States float [sequences,H,D,DV].  cu_seqlens NULL: `sequences` rows of n positions.  Packed: one row of n positions,
+ * cu_seqlens device int32 [sequences+1]; document i is [cu[i], cu[i+1]), any length, empty ones included.  The library cannot
+ * read the table on the host: entries are clamped to [0, n], so no table reaches outside the tensors, but the results are
+ * defined only for ascending ones; rows of no document are not written.  initial_state NULL: zeros; final_state NULL: not wanted.
+ * With a final state the chain of chunks carries its operands as pairs of bf16 (16 bits), without one as single bf16.
+ * `saved`: dism_delta_saved bytes, 256-byte aligned; dead after the call unless `backward` is set: then dism_delta_backward
+ * of the same call takes it (a size computed with final_state serves both). */
+size_t dism_delta_saved(int packed, int sequences, int n, int heads, int d, int dv, int final_state, int backward);
+int dism_delta_forward(const void *q, const void *k, const void *v, const void *g, const void *beta, int gates_bf16,
+                       const float *initial_state, const int32_t *cu_seqlens, int sequences, int n, int key_heads, int heads,
+                       int d, int dv, float scale, void *out, float *final_state, int backward, void *saved,
+                       size_t saved_bytes, void *stream);
+
+/* Its gradients: dq, dk bf16 [B,N,HK,D] (summed over the value heads of a key head), dv bf16 [B,N,H,DV], dg and dbeta [B,N,H] in the
+ * gates' type, dinitial_state float or NULL; dfinal_state is the gradient of the final state or NULL.  q and k are the forward's.
+ * Sums have a fixed order: results do not depend on the run. */
+size_t dism_delta_backward_workspace(int packed, int sequences, int n, int heads, int d, int dv);
+int dism_delta_backward(const void *q, const void *k, const void *dout, const float *dfinal_state, int gates_bf16,
+                        const int32_t *cu_seqlens, int sequences, int n, int key_heads, int heads, int d, int dv, float scale,
+                        const void *saved, size_t saved_bytes, void *dq, void *dk, void *dv_out, void *dg, void *dbeta,
+                        float *dinitial_state, void *workspace, size_t workspace_bytes, void *stream);
+
+/* One token per row, state updated in place: q, k bf16 [batch,HK,D], v, out bf16 [batch,H,DV], g, beta [batch,H],
+ * state float [pool,H,D,DV].  slots device int32 [batch]: the state of each row, or NULL for state i at row i.  A slot outside
+ * [0, pool) marks a row without a sequence: its output is zero.  Rows that name one slot are taken in order, as consecutive
+ * tokens of that sequence. */
+int dism_delta_step(const void *q, const void *k, const void *v, const void *g, const void *beta, int gates_bf16, float *state,
+                    const int32_t *slots, int64_t pool, int batch, int key_heads, int heads, int d, int dv, float scale,
+                    void *out, void *stream);
+
+/* Dropout: out[i] = (residual ? residual[i] : 0) + (r_i >= threshold ? x[i] * 65536 / (65536 - threshold) : 0), r_i the i-th 16-bit
+ * number of Philox4x32-10 with key seed[0] and counter (i / 8, site, seed[1]); seed is device int64 [2], read when the kernel
+ * runs.  type: 0 float, 1 half, 2 bf16.  The mask is not stored: the backward is this call on the gradient with residual NULL.
+ * out does not overlap x or residual.  No counterpart in the reference. */
+int dism_dropout(int type, const void *x, const void *residual, int64_t count, int threshold, const int64_t *seed, uint32_t site,
+                 void *out, void *stream);
+
 /* Per-kernel device timing for benchmarks (no counterpart in the reference, which times whole
  * calls with CUDA events from Python).  dism_profile_enable(1) clears the records and makes every
  * later launch record CUDA events around each kernel on its launch stream;
