@@ -19,14 +19,14 @@ namespace {
 
 template <int D, int WARPS>
 struct ReverseStage {
-    static constexpr int PITCH = 2 * D + 16, VALUE_PITCH = 32 * WARPS + 16;
+    static constexpr int PITCH = 2 * D, VALUE_PITCH = 32 * WARPS;
     static constexpr int K = 0, Q = K + CHUNK * PITCH, T = Q + CHUNK * PITCH, P = T + 2 * MATRIX;
-    static constexpr int DOUT = P + 2 * MATRIX, X = DOUT + CHUNK * VALUE_PITCH, ROWS = X + CHUNK * VALUE_PITCH;
-    static constexpr int BYTES = ROWS + 3 * CHUNK * 4;
+    static constexpr int DOUT = P + 2 * MATRIX, ROWS = DOUT + CHUNK * VALUE_PITCH, BYTES = ROWS + 3 * CHUNK * 4;
+    static constexpr int X = 2 * BYTES, TOTAL = X + CHUNK * VALUE_PITCH;  // one X for both stages: its columns belong to a warp each
 };
 
 template <int D, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) delta_reverse_kernel(DeltaShape shape, const __nv_bfloat16* __restrict__ q,
+__global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape shape, const __nv_bfloat16* __restrict__ q,
                                                                    const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ dout,
                                                                    const float* __restrict__ dfinal, DeltaSaved saved,
                                                                    __nv_bfloat16* __restrict__ dstates, float* __restrict__ dbeta_parts,
@@ -48,16 +48,14 @@ __global__ void __launch_bounds__(WARPS * 32) delta_reverse_kernel(DeltaShape sh
         const int count = min(CHUNK, length - c * CHUNK);
         const int64_t at = row + int64_t(c) * CHUNK, place = (slot + c) * shape.heads + head;
         const int64_t key = (at * shape.key_heads + key_head) * D * 2;
-        load_rows<2 * D, THREADS>(stage + Stage::K, Stage::PITCH, reinterpret_cast<const char*>(k) + key, key_stride, count, thread);
-        load_rows<32 * WARPS, THREADS>(stage + Stage::DOUT, Stage::VALUE_PITCH,
+        load_tile<2 * D, THREADS>(stage + Stage::K, reinterpret_cast<const char*>(k) + key, key_stride, count, thread);
+        load_tile<32 * WARPS, THREADS>(stage + Stage::DOUT,
                                        reinterpret_cast<const char*>(dout) + ((at * shape.heads + head) * dv + blockIdx.z * WARPS * 16) * 2,
                                        value_stride, count, thread);
         load_block<3 * CHUNK * 4, THREADS>(stage + Stage::ROWS, reinterpret_cast<const char*>(saved.rows + place * ROW_VALUES), thread);
         load_block<2 * MATRIX, THREADS>(stage + Stage::P, reinterpret_cast<const char*>(saved.p + place * MATRIX), thread);
         load_block<2 * MATRIX, THREADS>(stage + Stage::T, reinterpret_cast<const char*>(saved.t + place * MATRIX), thread);
-        load_rows<32 * WARPS, THREADS>(stage + Stage::X, Stage::VALUE_PITCH,
-                                       reinterpret_cast<const char*>(saved.x + place * CHUNK * dv + blockIdx.z * WARPS * 16), int64_t(dv) * 2, CHUNK, thread);
-        load_rows<2 * D, THREADS>(stage + Stage::Q, Stage::PITCH, reinterpret_cast<const char*>(q) + key, key_stride, count, thread);
+        load_tile<2 * D, THREADS>(stage + Stage::Q, reinterpret_cast<const char*>(q) + key, key_stride, count, thread);
         cp_async_commit();
     };
 
@@ -72,7 +70,18 @@ __global__ void __launch_bounds__(WARPS * 32) delta_reverse_kernel(DeltaShape sh
     for (int c = chunks - 1; c >= 0; --c) {
         cp_async_wait<0>();
         __syncthreads();  // chunk c is in, and every warp has left chunk c + 1
+        {  // X of this chunk: the warp's own columns, needed only after dU
+            const char* from = reinterpret_cast<const char*>(saved.x + ((slot + c) * shape.heads + head) * CHUNK * dv + column) + (lane & 1) * 16;
+#pragma unroll
+            for (int i = 0; i < CHUNK * 2 / 32; ++i) {
+                const int t = i * 16 + (lane >> 1);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + Stage::X + t * Stage::VALUE_PITCH + ((warp * 2 + (lane & 1)) ^ piece_key<Stage::VALUE_PITCH>(t)) * 16),
+                             "l"(from + int64_t(t) * dv * 2));
+            }
+            cp_async_commit();
+        }
         if (c > 0) load(c - 1);
+        else cp_async_commit();
         const unsigned stage = base + (c & 1) * Stage::BYTES;
         const float* rows = reinterpret_cast<const float*>(shared + (c & 1) * Stage::BYTES + Stage::ROWS);
         const int64_t place = (slot + c) * shape.heads + head;
@@ -82,7 +91,7 @@ __global__ void __launch_bounds__(WARPS * 32) delta_reverse_kernel(DeltaShape sh
         for (int n = 0; n < TILES; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) du[n][e] = 0.f;
-        const unsigned keys = stage + Stage::K + cols_first(lane, Stage::PITCH);
+        const TileLane keys = tile_cols_first<Stage::PITCH>(stage + Stage::K, lane);
         unsigned* state_out = reinterpret_cast<unsigned*>(dstates + place * dv * D) + int64_t(column / 8) * (D / 8) * 32 + lane;
 #pragma unroll
         for (int kb = 0; kb < D / 16; ++kb) {
@@ -93,12 +102,12 @@ __global__ void __launch_bounds__(WARPS * 32) delta_reverse_kernel(DeltaShape sh
 #pragma unroll
             for (int np = 0; np < TILES / 2; ++np) {
                 unsigned b[4];
-                ldsm4(b, keys + np * 16 * Stage::PITCH + kb * 32);
+                ldsm4(b, keys.at(kb * 32) + np * 16 * Stage::PITCH);
                 mma16816(du[2 * np], a, b[0], b[1]);
                 mma16816(du[2 * np + 1], a, b[2], b[3]);
             }
         }
-        const unsigned own = warp * 32 + cols_first(lane, Stage::VALUE_PITCH);
+        const unsigned own = tile_cols_first<Stage::VALUE_PITCH>(0, lane).at(warp * 32), values = base + Stage::X + own;
         unsigned grad[TILES / 2][4];  // dO, transposed, as a left operand
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np) {
@@ -110,23 +119,25 @@ __global__ void __launch_bounds__(WARPS * 32) delta_reverse_kernel(DeltaShape sh
                 tile[0] *= tail.x, tile[1] *= tail.y, tile[2] *= tail.x, tile[3] *= tail.y;
             }
         }
-        const unsigned inside = stage + Stage::P + rows_first_blocked(lane, TILES), inverse = inside + Stage::T - Stage::P;
+        const unsigned inside = stage + Stage::P + rows_first_tile(lane), inverse = inside + Stage::T - Stage::P;
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np)
 #pragma unroll
             for (int kb = np; kb < TILES / 2; ++kb) {
                 unsigned b[4];
-                ldsm4_trans(b, inside + (kb * 2 * TILES + np * 2) * 128);
+                ldsm4_trans(b, inside + tile_at(kb, np));
                 mma16816(du[2 * np], grad[kb], b[0], b[1]);
                 mma16816(du[2 * np + 1], grad[kb], b[2], b[3]);
             }
         // the part of db that needs dU: this warp's 16 columns of dU.X
         float* part = dbeta_parts + (int64_t(column / 16) * shape.layout.slots() * shape.heads + place) * CHUNK;
         unsigned dx[TILES / 2][4];
+        cp_async_wait<1>();  // all but the next chunk
+        __syncwarp();
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np) {
             unsigned xx[4];
-            ldsm4_trans(xx, stage + Stage::X + own + np * 16 * Stage::VALUE_PITCH);
+            ldsm4_trans(xx, values + np * 16 * Stage::VALUE_PITCH);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float(&tile)[4] = du[2 * np + h];
@@ -150,12 +161,11 @@ __global__ void __launch_bounds__(WARPS * 32) delta_reverse_kernel(DeltaShape sh
 #pragma unroll
             for (int kb = np; kb < TILES / 2; ++kb) {
                 unsigned b[4];
-                ldsm4_trans(b, inverse + (kb * 2 * TILES + np * 2) * 128);
+                ldsm4_trans(b, inverse + tile_at(kb, np));
                 mma16816(dy[2 * np], dx[kb], b[0], b[1]);
                 mma16816(dy[2 * np + 1], dx[kb], b[2], b[3]);
             }
         // dV leaves through the warp's columns of the X tile
-        const unsigned values = stage + Stage::X + own;
         __syncwarp();
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np)
@@ -167,9 +177,10 @@ __global__ void __launch_bounds__(WARPS * 32) delta_reverse_kernel(DeltaShape sh
 #pragma unroll
         for (int i = 0; i < CHUNK * 2 / 32; ++i) {
             const int t = i * 16 + (lane >> 1);
-            const uint4 piece = *reinterpret_cast<const uint4*>(shared + (c & 1) * Stage::BYTES + Stage::X + t * Stage::VALUE_PITCH + warp * 32 + (lane & 1) * 16);
+            const uint4 piece = *reinterpret_cast<const uint4*>(shared + Stage::X + t * Stage::VALUE_PITCH + ((warp * 2 + (lane & 1)) ^ piece_key<Stage::VALUE_PITCH>(t)) * 16);
             if (t < count) *reinterpret_cast<uint4*>(to + t * value_stride + (lane & 1) * 16) = piece;
         }
+        __syncwarp();  // the columns are free for the next chunk's X
         // scale e^G dO and -e^G dY, the left operands of the state's step
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np) {
@@ -190,16 +201,16 @@ __global__ void __launch_bounds__(WARPS * 32) delta_reverse_kernel(DeltaShape sh
         for (int n = 0; n < D / 8; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) ds[n][e] *= kept;
-        const unsigned keys_trans = stage + Stage::K + rows_first(lane, Stage::PITCH), queries_trans = keys_trans + Stage::Q - Stage::K;
+        const TileLane keys_trans = tile_rows_first<Stage::PITCH>(stage + Stage::K, lane);
 #pragma unroll
         for (int kb = 0; kb < TILES / 2; ++kb)
 #pragma unroll
             for (int np = 0; np < D / 16; ++np) {
                 unsigned b[4];
-                ldsm4_trans(b, keys_trans + kb * 16 * Stage::PITCH + np * 32);
+                ldsm4_trans(b, keys_trans.at(np * 32) + kb * 16 * Stage::PITCH);
                 mma16816(ds[2 * np], dx[kb], b[0], b[1]);
                 mma16816(ds[2 * np + 1], dx[kb], b[2], b[3]);
-                ldsm4_trans(b, queries_trans + kb * 16 * Stage::PITCH + np * 32);
+                ldsm4_trans(b, keys_trans.at(np * 32) + Stage::Q - Stage::K + kb * 16 * Stage::PITCH);
                 mma16816(ds[2 * np], grad[kb], b[0], b[1]);
                 mma16816(ds[2 * np + 1], grad[kb], b[2], b[3]);
             }
@@ -527,7 +538,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_kernel(Del
 
 template <int D, int WARPS>
 cudaError_t launch_reverse(const DeltaShape& shape, const DeltaGradients& x, const DeltaSaved& saved, cudaStream_t stream) {
-    constexpr int BYTES = 2 * ReverseStage<D, WARPS>::BYTES;
+    constexpr int BYTES = ReverseStage<D, WARPS>::TOTAL;
     auto* kernel = delta_reverse_kernel<D, WARPS>;
     if (cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES)) return status;
     KernelTimer timer("delta_reverse", stream);

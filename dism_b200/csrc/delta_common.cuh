@@ -21,7 +21,7 @@ namespace dism {
 
 constexpr int CHUNK = 64;
 constexpr int ROW_VALUES = 5 * CHUNK;      // per chunk and head: decay, beta, tail, and G as a pair of floats
-constexpr int MATRIX = CHUNK * CHUNK;      // elements of T and P of one chunk and head
+constexpr int MATRIX = 10 * 256;           // elements of T and P of one chunk and head: the 16 x 16 tiles up to the diagonal
 constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
@@ -66,10 +66,13 @@ __device__ __forceinline__ void to_operand_rest(unsigned (&r)[4], const unsigned
 // cols_first: the two middle ones exchanged.
 __device__ __forceinline__ unsigned rows_first(int lane, int pitch) { return ((lane & 7) + (lane & 8)) * pitch + (lane >> 4) * 16; }
 __device__ __forceinline__ unsigned cols_first(int lane, int pitch) { return ((lane & 7) + ((lane >> 4) << 3)) * pitch + ((lane >> 3) & 1) * 16; }
-// The same for matrices stored as 8 x 8 blocks of 128 contiguous bytes, `width` blocks to a row of blocks (how the kernels
-// keep T, P and the states between each other: fragments leave and enter in whole lines and no access has a bank conflict).
+// The kernels hand T, P and the states to one another as 8 x 8 blocks of 128 contiguous bytes: fragments leave and enter in whole
+// lines and no access has a bank conflict.  States: `width` blocks to a row of blocks.  T and P: 16 x 16 tiles of four blocks, by
+// rows, the tiles on and below the diagonal one after the other.
 __device__ __forceinline__ unsigned rows_first_blocked(int lane, int width) { return (((lane >> 3) & 1) * width + (lane >> 4)) * 128 + (lane & 7) * 16; }
-__device__ __forceinline__ unsigned cols_first_blocked(int lane, int width) { return ((lane >> 4) * width + ((lane >> 3) & 1)) * 128 + (lane & 7) * 16; }
+__device__ __forceinline__ unsigned rows_first_tile(int lane) { return rows_first_blocked(lane, 2); }
+__device__ __forceinline__ unsigned cols_first_tile(int lane) { return lane * 16; }
+__host__ __device__ constexpr int tile_at(int row_tile, int column_tile) { return (row_tile * (row_tile + 1) / 2 + column_tile) * 512; }
 
 // Where the sequences lie.  Fixed layout: `sequences` rows of n positions.  Packed: one row of n positions, document i at
 // [cu[i], cu[i+1]).  Every chunk has a slot of its own: in a pack, document i starts at slot cu[i] / 64 + i, which leaves
@@ -130,7 +133,52 @@ __device__ __forceinline__ float gate(const void* gates, int64_t index, bool is_
     return is_bf16 ? bf2f(static_cast<const __nv_bfloat16*>(gates)[index]) : static_cast<const float*>(gates)[index];
 }
 
-// Copies `count` rows of `bytes` bytes (a multiple of 16) from a strided tensor into a padded tile of 64 rows; the rest is zeros.
+// Tiles of 64 rows of BYTES bytes in shared memory: the 16-byte pieces of a row are exchanged by the row number, so that the eight
+// rows of an ldmatrix fall into different banks without padding.
+template <int BYTES>
+__device__ __forceinline__ int piece_key(int row) { return BYTES >= 128 ? row & 7 : (row >> 1) & 3; }
+// A lane's view of such a tile for ldmatrix / stmatrix: `at` + its row, and what its pieces are exchanged by.  A 16 x 16 part that
+// starts at row 16 i and piece 2 j is at row + 16 i * BYTES + ((32 j) ^ flip).
+struct TileLane {
+    unsigned row, flip;
+    __device__ __forceinline__ unsigned at(int bytes) const { return row + (unsigned(bytes) ^ flip); }
+};
+template <int BYTES>
+__device__ __forceinline__ TileLane tile_rows_first(unsigned tile, int lane) {
+    const int row = (lane & 7) + (lane & 8);
+    return {tile + row * BYTES, unsigned(((lane >> 4) ^ piece_key<BYTES>(row)) * 16)};
+}
+template <int BYTES>
+__device__ __forceinline__ TileLane tile_cols_first(unsigned tile, int lane) {
+    const int row = (lane & 7) + ((lane >> 4) << 3);
+    return {tile + row * BYTES, unsigned((((lane >> 3) & 1) ^ piece_key<BYTES>(row)) * 16)};
+}
+// Copies `count` rows from a strided tensor into such a tile; the rest is zeros.  A full chunk takes the unrolled path with one
+// running pointer: addresses worked out ahead of the loop over the chunks would cost the chains their registers.
+template <int BYTES, int THREADS>
+__device__ __forceinline__ void load_tile(unsigned tile, const char* global, int64_t stride, int count, int thread) {
+    constexpr int PIECES = BYTES / 16, STEP = THREADS / PIECES;  // rows that the threads take at a time
+    static_assert(THREADS % PIECES == 0 && CHUNK % STEP == 0 && (STEP % 8 == 0 || 8 % STEP == 0), "rows are dealt out evenly");
+    const int first = thread / PIECES, piece = thread % PIECES;
+    const char* from = global + first * stride + piece * 16;
+    const unsigned to = tile + first * BYTES;
+    if (count == CHUNK) {
+#pragma unroll
+        for (int row = 0; row < CHUNK; row += STEP) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + row * BYTES + ((piece ^ piece_key<BYTES>(first + row)) * 16)), "l"(from) : "memory");
+            from += STEP * stride;
+        }
+    } else {
+#pragma unroll 1
+        for (int row = 0; row < CHUNK; row += STEP) {
+            const bool inside = first + row < count;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + row * BYTES + ((piece ^ piece_key<BYTES>(first + row)) * 16)),
+                         "l"(inside ? from : global), "r"(inside ? 16 : 0) : "memory");
+            from += STEP * stride;
+        }
+    }
+}
+// The same with padded rows of `pitch` bytes.
 template <int BYTES, int THREADS>
 __device__ __forceinline__ void load_rows(unsigned tile, int pitch, const char* global, int64_t stride, int count, int thread) {
     constexpr int PIECES = BYTES / 16;

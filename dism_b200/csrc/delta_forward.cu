@@ -14,14 +14,14 @@ namespace {
 
 template <int D, int WARPS, bool EXACT>
 struct ForwardStage {
-    static constexpr int PITCH = 2 * D + 16, VALUE_PITCH = 32 * WARPS + 16;
+    static constexpr int PITCH = 2 * D, VALUE_PITCH = 32 * WARPS;
     static constexpr int K = 0, Q = K + CHUNK * PITCH, T = Q + CHUNK * PITCH, T_REST = T + 2 * MATRIX;
     static constexpr int P = T_REST + (EXACT ? 2 * MATRIX : 0), V = P + 2 * MATRIX, ROWS = V + CHUNK * VALUE_PITCH;
     static constexpr int BYTES = ROWS + 3 * CHUNK * 4;
 };
 
 template <int D, int WARPS, bool EXACT, bool SAVE>
-__global__ void __launch_bounds__(WARPS * 32) delta_chain_kernel(DeltaShape shape, const __nv_bfloat16* __restrict__ q,
+__global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape shape, const __nv_bfloat16* __restrict__ q,
                                                                  const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v,
                                                                  const float* __restrict__ initial, DeltaSaved saved,
                                                                  __nv_bfloat16* __restrict__ out, float* __restrict__ final_state) {
@@ -43,14 +43,14 @@ __global__ void __launch_bounds__(WARPS * 32) delta_chain_kernel(DeltaShape shap
         const int count = min(CHUNK, length - c * CHUNK);
         const int64_t at = row + int64_t(c) * CHUNK, place = (slot + c) * shape.heads + head;
         const int64_t key = (at * shape.key_heads + key_head) * D * 2;
-        load_rows<2 * D, THREADS>(stage + Stage::K, Stage::PITCH, reinterpret_cast<const char*>(k) + key, key_stride, count, thread);
-        load_rows<32 * WARPS, THREADS>(stage + Stage::V, Stage::VALUE_PITCH,
+        load_tile<2 * D, THREADS>(stage + Stage::K, reinterpret_cast<const char*>(k) + key, key_stride, count, thread);
+        load_tile<32 * WARPS, THREADS>(stage + Stage::V,
                                        reinterpret_cast<const char*>(v) + ((at * shape.heads + head) * dv + blockIdx.z * WARPS * 16) * 2,
                                        value_stride, count, thread);
         load_block<3 * CHUNK * 4, THREADS>(stage + Stage::ROWS, reinterpret_cast<const char*>(saved.rows + place * ROW_VALUES), thread);
         load_block<2 * MATRIX, THREADS>(stage + Stage::T, reinterpret_cast<const char*>(saved.t + place * MATRIX), thread);
         if (EXACT) load_block<2 * MATRIX, THREADS>(stage + Stage::T_REST, reinterpret_cast<const char*>(saved.t_rest + place * MATRIX), thread);
-        load_rows<2 * D, THREADS>(stage + Stage::Q, Stage::PITCH, reinterpret_cast<const char*>(q) + key, key_stride, count, thread);
+        load_tile<2 * D, THREADS>(stage + Stage::Q, reinterpret_cast<const char*>(q) + key, key_stride, count, thread);
         load_block<2 * MATRIX, THREADS>(stage + Stage::P, reinterpret_cast<const char*>(saved.p + place * MATRIX), thread);
         cp_async_commit();
     };
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(WARPS * 32) delta_chain_kernel(DeltaShape shap
         for (int n = 0; n < TILES; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) ks[n][e] = qs[n][e] = 0.f;
-        const unsigned keys = stage + Stage::K + cols_first(lane, Stage::PITCH), queries = keys + Stage::Q - Stage::K;
+        const TileLane keys = tile_cols_first<Stage::PITCH>(stage + Stage::K, lane);
 #pragma unroll
         for (int kb = 0; kb < D / 16; ++kb) {
             unsigned a[4], rest[4];
@@ -89,20 +89,20 @@ __global__ void __launch_bounds__(WARPS * 32) delta_chain_kernel(DeltaShape shap
 #pragma unroll
             for (int np = 0; np < TILES / 2; ++np) {
                 unsigned b[4];
-                ldsm4(b, keys + np * 16 * Stage::PITCH + kb * 32);
+                ldsm4(b, keys.at(kb * 32) + np * 16 * Stage::PITCH);
                 mma16816(ks[2 * np], a, b[0], b[1]);
                 mma16816(ks[2 * np + 1], a, b[2], b[3]);
                 if (EXACT) {
                     mma16816(ks[2 * np], rest, b[0], b[1]);
                     mma16816(ks[2 * np + 1], rest, b[2], b[3]);
                 }
-                ldsm4(b, queries + np * 16 * Stage::PITCH + kb * 32);
+                ldsm4(b, keys.at(kb * 32) + Stage::Q - Stage::K + np * 16 * Stage::PITCH);
                 mma16816(qs[2 * np], a, b[0], b[1]);
                 mma16816(qs[2 * np + 1], a, b[2], b[3]);
             }
         }
         // Y, as the left operand of X = T Y
-        const unsigned values = stage + Stage::V + warp * 32 + cols_first(lane, Stage::VALUE_PITCH);
+        const unsigned values = tile_cols_first<Stage::VALUE_PITCH>(stage + Stage::V, lane).at(warp * 32);
         unsigned y[TILES / 2][4], y_rest[EXACT ? TILES / 2 : 1][4];
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np) {
@@ -126,19 +126,19 @@ __global__ void __launch_bounds__(WARPS * 32) delta_chain_kernel(DeltaShape shap
         for (int n = 0; n < TILES; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[n][e] = 0.f;
-        const unsigned inverse = stage + Stage::T + cols_first_blocked(lane, TILES), inside = inverse + Stage::P - Stage::T;
+        const unsigned inverse = stage + Stage::T + cols_first_tile(lane), inside = inverse + Stage::P - Stage::T;
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np)
 #pragma unroll
             for (int kb = 0; kb <= np; ++kb) {
                 unsigned b[4];
-                ldsm4(b, inverse + (np * 2 * TILES + kb * 2) * 128);
+                ldsm4(b, inverse + tile_at(np, kb));
                 mma16816(x[2 * np], y[kb], b[0], b[1]);
                 mma16816(x[2 * np + 1], y[kb], b[2], b[3]);
                 if (EXACT) {
                     mma16816(x[2 * np], y_rest[kb], b[0], b[1]);
                     mma16816(x[2 * np + 1], y_rest[kb], b[2], b[3]);
-                    ldsm4(b, inverse + Stage::T_REST - Stage::T + (np * 2 * TILES + kb * 2) * 128);
+                    ldsm4(b, inverse + Stage::T_REST - Stage::T + tile_at(np, kb));
                     mma16816(x[2 * np], y[kb], b[0], b[1]);
                     mma16816(x[2 * np + 1], y[kb], b[2], b[3]);
                 }
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(WARPS * 32) delta_chain_kernel(DeltaShape shap
 #pragma unroll
             for (int i = 0; i < CHUNK * 2 / 32; ++i) {
                 const int t = i * 16 + (lane >> 1);
-                const uint4 piece = *reinterpret_cast<const uint4*>(shared + (c & 1) * Stage::BYTES + Stage::V + t * Stage::VALUE_PITCH + warp * 32 + (lane & 1) * 16);
+                const uint4 piece = *reinterpret_cast<const uint4*>(shared + (c & 1) * Stage::BYTES + Stage::V + t * Stage::VALUE_PITCH + ((warp * 2 + (lane & 1)) ^ piece_key<Stage::VALUE_PITCH>(t)) * 16);
                 if (t < rows_out) *reinterpret_cast<uint4*>(to + t * stride + (lane & 1) * 16) = piece;
             }
         };
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(WARPS * 32) delta_chain_kernel(DeltaShape shap
 #pragma unroll
             for (int kb = 0; kb <= np; ++kb) {
                 unsigned b[4];
-                ldsm4(b, inside + (np * 2 * TILES + kb * 2) * 128);
+                ldsm4(b, inside + tile_at(np, kb));
                 mma16816(qs[2 * np], u[kb], b[0], b[1]);
                 mma16816(qs[2 * np + 1], u[kb], b[2], b[3]);
             }
@@ -199,13 +199,13 @@ __global__ void __launch_bounds__(WARPS * 32) delta_chain_kernel(DeltaShape shap
         for (int n = 0; n < D / 8; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[n][e] *= kept;
-        const unsigned keys_trans = stage + Stage::K + rows_first(lane, Stage::PITCH);
+        const TileLane keys_trans = tile_rows_first<Stage::PITCH>(stage + Stage::K, lane);
 #pragma unroll
         for (int kb = 0; kb < TILES / 2; ++kb)
 #pragma unroll
             for (int np = 0; np < D / 16; ++np) {
                 unsigned b[4];
-                ldsm4_trans(b, keys_trans + kb * 16 * Stage::PITCH + np * 32);
+                ldsm4_trans(b, keys_trans.at(np * 32) + kb * 16 * Stage::PITCH);
                 mma16816(s[2 * np], u[kb], b[0], b[1]);
                 mma16816(s[2 * np + 1], u[kb], b[2], b[3]);
                 if (EXACT) {
