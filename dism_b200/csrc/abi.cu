@@ -402,6 +402,11 @@ int dism_delta_backward(const void* q, const void* k, const void* dout, const fl
     return cuda_status(dism::launch_delta_backward(shape, x, parts, static_cast<cudaStream_t>(stream)), "delta_backward");
 }
 
+int dism_delta_fault(int* code) {
+    if (!code) return fail(DISM_EINVAL, "null pointer");
+    return cuda_status(dism::read_delta_fault(code), "delta fault code");
+}
+
 int dism_delta_step(const void* q, const void* k, const void* v, const void* g, const void* beta, int gates_bf16, float* state,
                     const int32_t* slots, int64_t pool, int batch, int key_heads, int heads, int d, int dv, float scale, void* out,
                     void* stream) {

@@ -70,14 +70,11 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
     for (int c = chunks - 1; c >= 0; --c) {
         cp_async_wait<0>();
         __syncthreads();  // chunk c is in, and every warp has left chunk c + 1
-        {  // X of this chunk: the warp's own columns, needed only after dU
-            const char* from = reinterpret_cast<const char*>(saved.x + ((slot + c) * shape.heads + head) * CHUNK * dv + column) + (lane & 1) * 16;
+        {  // X of this chunk, transposed: the warp's own rows, two kilobytes, needed only after dU
+            const char* from = reinterpret_cast<const char*>(saved.x + ((slot + c) * shape.heads + head) * CHUNK * dv + column * CHUNK);
 #pragma unroll
-            for (int i = 0; i < CHUNK * 2 / 32; ++i) {
-                const int t = i * 16 + (lane >> 1);
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + Stage::X + t * Stage::VALUE_PITCH + ((warp * 2 + (lane & 1)) ^ piece_key<Stage::VALUE_PITCH>(t)) * 16),
-                             "l"(from + int64_t(t) * dv * 2));
-            }
+            for (int i = lane * 16; i < 2048; i += 512)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + Stage::X + warp * 2048 + i), "l"(from + i));
             cp_async_commit();
         }
         if (c > 0) load(c - 1);
@@ -107,7 +104,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
                 mma16816(du[2 * np + 1], a, b[2], b[3]);
             }
         }
-        const unsigned own = tile_cols_first<Stage::VALUE_PITCH>(0, lane).at(warp * 32), values = base + Stage::X + own;
+        const unsigned own = tile_cols_first<Stage::VALUE_PITCH>(0, lane).at(warp * 32);
         unsigned grad[TILES / 2][4];  // dO, transposed, as a left operand
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np) {
@@ -137,7 +134,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np) {
             unsigned xx[4];
-            ldsm4_trans(xx, values + np * 16 * Stage::VALUE_PITCH);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) xx[e] = *reinterpret_cast<const unsigned*>(shared + Stage::X + warp * 2048 + ((e & 1) * TILES + 2 * np + (e >> 1)) * 128 + lane * 4);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float(&tile)[4] = du[2 * np + h];
@@ -165,11 +163,12 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
                 mma16816(dy[2 * np], dx[kb], b[0], b[1]);
                 mma16816(dy[2 * np + 1], dx[kb], b[2], b[3]);
             }
-        // dV leaves through the warp's columns of the X tile
+        // dV leaves through the warp's room of X: rows of 32 bytes, the halves of rows 4-7 of every eight exchanged
+        const unsigned values = base + Stage::X + warp * 2048 + ((lane & 7) + ((lane >> 4) << 3)) * 32 + ((((lane >> 3) ^ (lane >> 2)) & 1) * 16);
         __syncwarp();
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np)
-            stsm4_trans(values + np * 16 * Stage::VALUE_PITCH, pack2(dy[2 * np][0], dy[2 * np][1]), pack2(dy[2 * np][2], dy[2 * np][3]),
+            stsm4_trans(values + np * 512, pack2(dy[2 * np][0], dy[2 * np][1]), pack2(dy[2 * np][2], dy[2 * np][3]),
                         pack2(dy[2 * np + 1][0], dy[2 * np + 1][1]), pack2(dy[2 * np + 1][2], dy[2 * np + 1][3]));
         __syncwarp();
         const int count = min(CHUNK, length - c * CHUNK);
@@ -177,10 +176,10 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
 #pragma unroll
         for (int i = 0; i < CHUNK * 2 / 32; ++i) {
             const int t = i * 16 + (lane >> 1);
-            const uint4 piece = *reinterpret_cast<const uint4*>(shared + Stage::X + t * Stage::VALUE_PITCH + ((warp * 2 + (lane & 1)) ^ piece_key<Stage::VALUE_PITCH>(t)) * 16);
+            const uint4 piece = *reinterpret_cast<const uint4*>(shared + Stage::X + warp * 2048 + t * 32 + (((lane & 1) ^ ((t >> 2) & 1)) * 16));
             if (t < count) *reinterpret_cast<uint4*>(to + t * value_stride + (lane & 1) * 16) = piece;
         }
-        __syncwarp();  // the columns are free for the next chunk's X
+        __syncwarp();  // the room is free for the next chunk's X
         // scale e^G dO and -e^G dY, the left operands of the state's step
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np) {
@@ -230,7 +229,7 @@ template <int D, int DV>
 struct GradientShared {
     static constexpr int PITCH = 2 * D + 16, VALUE_PITCH = 2 * DV + 16, MATRIX_PITCH = 2 * CHUNK + 16;
     static constexpr int K = 0, Q = K + CHUNK * PITCH, DOUT = Q + CHUNK * PITCH, DY = DOUT + CHUNK * VALUE_PITCH, X = DY + CHUNK * VALUE_PITCH;
-    static constexpr int S0 = X + CHUNK * VALUE_PITCH, DS = S0 + 2 * D * DV, DP = DS + 2 * D * DV, DL = DP + CHUNK * MATRIX_PITCH;
+    static constexpr int S0 = X + CHUNK * 2 * DV, DS = S0 + 2 * D * DV, DP = DS + 2 * D * DV, DL = DP + CHUNK * MATRIX_PITCH;
     static constexpr int ROWS = DL + CHUNK * MATRIX_PITCH, SUMS = ROWS + ROW_VALUES * 4;
     // sums: rows of M [2][64], columns of M [4][2][64], columns of b [4][64], state terms of dG [2][64] and dG_63 [2][64], <dS1, S0> [8]
     static constexpr int ROW_SUM = 0, COLUMN_SUM = ROW_SUM + 2 * CHUNK, BETA_SUM = COLUMN_SUM + 8 * CHUNK, STATE_SUM = BETA_SUM + 4 * CHUNK;
@@ -271,7 +270,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_kernel(Del
     for (int head = key_head * group; head < (key_head + 1) * group; ++head) {
         const int64_t place = slot * shape.heads + head;
         const int64_t value = (row * shape.heads + head) * DV * 2;
-        load_rows<2 * DV, GRADIENT_THREADS>(base + Shared::X, Shared::VALUE_PITCH, reinterpret_cast<const char*>(saved.x + place * CHUNK * DV), DV * 2, CHUNK, thread);
+        load_block<2 * CHUNK * DV, GRADIENT_THREADS>(base + Shared::X, reinterpret_cast<const char*>(saved.x + place * CHUNK * DV), thread);
         load_rows<2 * DV, GRADIENT_THREADS>(base + Shared::DOUT, Shared::VALUE_PITCH, reinterpret_cast<const char*>(dout) + value, value_stride, count, thread);
         load_rows<2 * DV, GRADIENT_THREADS>(base + Shared::DY, Shared::VALUE_PITCH, reinterpret_cast<const char*>(dy) + value, value_stride, count, thread);
         load_block<ROW_VALUES * 4, GRADIENT_THREADS>(base + Shared::ROWS, reinterpret_cast<const char*>(saved.rows + place * ROW_VALUES), thread);
@@ -288,7 +287,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_kernel(Del
 #pragma unroll
                 for (int e = 0; e < 4; ++e) z[n][e] = y[n][e] = 0.f;
             const unsigned own = base + (half ? Shared::DY : Shared::DOUT) + part * 16 * Shared::VALUE_PITCH + rows_first(lane, Shared::VALUE_PITCH);
-            const unsigned xs = base + Shared::X + cols_first(lane, Shared::VALUE_PITCH);
+            const unsigned xs = base + Shared::X + rows_first_blocked(lane, TILES);
 #pragma unroll
             for (int kb = 0; kb < DV / 16; ++kb) {
                 unsigned a[4];
@@ -297,7 +296,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_kernel(Del
                 for (int np = 0; np < TILES / 2; ++np) {
                     if (np > part) continue;
                     unsigned b[4];
-                    ldsm4(b, xs + np * 16 * Shared::VALUE_PITCH + kb * 32);
+                    ldsm4_trans(b, xs + (kb * 2 * TILES + np * 2) * 128);
                     mma16816(z[2 * np], a, b[0], b[1]);
                     mma16816(z[2 * np + 1], a, b[2], b[3]);
                 }
@@ -317,7 +316,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_kernel(Del
                     mma16816(y[2 * np + 1], a, b[2], b[3]);
                 }
             }
-            const float *high = rows + 3 * CHUNK, *low = rows + 4 * CHUNK, *beta = rows + CHUNK;
+            const float *high = rows + ROW_HIGH, *low = rows + ROW_LOW, *beta = rows + ROW_BETA;
             float row_sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int n = 0; n < TILES; ++n) {
@@ -381,17 +380,19 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_kernel(Del
         float state_sum[2] = {0.f, 0.f}, last_sum[2] = {0.f, 0.f};
         float tile[NT][4];
         // 16 rows of a value-wide operand times half of a state
-        auto state_product = [&](int operand, int state) {
+        auto state_product = [&](int operand, int state, bool transposed) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) tile[n][e] = 0.f;
-            const unsigned left = base + operand + part * 16 * Shared::VALUE_PITCH + rows_first(lane, Shared::VALUE_PITCH);
+            const unsigned left = transposed ? base + operand + cols_first_blocked(lane, TILES) + part * 256
+                                             : base + operand + part * 16 * Shared::VALUE_PITCH + rows_first(lane, Shared::VALUE_PITCH);
             const unsigned right = base + state + rows_first_blocked(lane, D / 8) + half * (D / 16) * 128;
 #pragma unroll
             for (int kb = 0; kb < DV / 16; ++kb) {
                 unsigned a[4];
-                ldsm4(a, left + kb * 32);
+                if (transposed) ldsm4_trans(a, left + kb * 2 * TILES * 128);
+                else ldsm4(a, left + kb * 32);
 #pragma unroll
                 for (int np = 0; np < NT / 2; ++np) {
                     unsigned b[4];
@@ -414,12 +415,12 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_kernel(Del
                 dots[1] += v2 * low_half(x1) + v3 * high_half(x1);
             }
         };
-        state_product(Shared::DOUT, Shared::S0);
+        state_product(Shared::DOUT, Shared::S0, false);
         take(dq_sum, Shared::Q, shape.scale * decay[0], shape.scale * decay[1], state_sum);
-        state_product(Shared::DY, Shared::S0);
+        state_product(Shared::DY, Shared::S0, false);
         take(dk_sum, Shared::K, -decay[0], -decay[1], state_sum);
-        state_product(Shared::X, Shared::DS);
-        take(dk_sum, Shared::K, rows[2 * CHUNK + t0] * rows[CHUNK + t0], rows[2 * CHUNK + t0 + 8] * rows[CHUNK + t0 + 8], last_sum);
+        state_product(Shared::X, Shared::DS, true);
+        take(dk_sum, Shared::K, rows[ROW_WRITE + t0], rows[ROW_WRITE + t0 + 8], last_sum);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
 #pragma unroll
@@ -513,7 +514,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_kernel(Del
                 if (t < count) {
                     const int64_t index = (row + t) * shape.heads + head;
                     // a decay that is zero in 32 bits has no gradient; the sum would leave the roundings of terms that cancel
-                    const float *high = rows + 3 * CHUNK, *low = rows + 4 * CHUNK;
+                    const float *high = rows + ROW_HIGH, *low = rows + ROW_LOW;
                     const float step = t ? (high[t] - high[t - 1]) + (low[t] - low[t - 1]) : high[0];
                     const float value = step < -149.f ? 0.f : after + here[e];
                     if (shape.gates_bf16) static_cast<__nv_bfloat16*>(dg)[index] = __float2bfloat16(value);
@@ -562,6 +563,7 @@ template <int D>
 cudaError_t launch_width(const DeltaShape& shape, const DeltaGradients& x, const DeltaSaved& saved, cudaStream_t stream) {
     cudaError_t status = shape.dv % 64 == 0 ? launch_reverse<D, 4>(shape, x, saved, stream) : launch_reverse<D, 2>(shape, x, saved, stream);
     if (status || shape.layout.slots() == 0) return status;
+    if (D >= 64 && shape.dv >= 64) return launch_delta_gradient_tensor(shape, x, saved, stream);
     if (shape.dv == 32) return launch_gradient<D, 32>(shape, x, saved, stream);
     if (shape.dv == 64) return launch_gradient<D, 64>(shape, x, saved, stream);
     return launch_gradient<D, 128>(shape, x, saved, stream);

@@ -20,7 +20,8 @@
 namespace dism {
 
 constexpr int CHUNK = 64;
-constexpr int ROW_VALUES = 5 * CHUNK;      // per chunk and head: decay, beta, tail, and G as a pair of floats
+// Per chunk and head: e^G, b, e^{G_63 - G}, the product of the last two, and G as a pair of floats.
+constexpr int ROW_DECAY = 0, ROW_BETA = CHUNK, ROW_TAIL = 2 * CHUNK, ROW_WRITE = 3 * CHUNK, ROW_HIGH = 4 * CHUNK, ROW_LOW = 5 * CHUNK, ROW_VALUES = 6 * CHUNK;
 constexpr int MATRIX = 10 * 256;           // elements of T and P of one chunk and head: the 16 x 16 tiles up to the diagonal
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -70,6 +71,7 @@ __device__ __forceinline__ unsigned cols_first(int lane, int pitch) { return ((l
 // lines and no access has a bank conflict.  States: `width` blocks to a row of blocks.  T and P: 16 x 16 tiles of four blocks, by
 // rows, the tiles on and below the diagonal one after the other.
 __device__ __forceinline__ unsigned rows_first_blocked(int lane, int width) { return (((lane >> 3) & 1) * width + (lane >> 4)) * 128 + (lane & 7) * 16; }
+__device__ __forceinline__ unsigned cols_first_blocked(int lane, int width) { return ((lane >> 4) * width + ((lane >> 3) & 1)) * 128 + (lane & 7) * 16; }
 __device__ __forceinline__ unsigned rows_first_tile(int lane) { return rows_first_blocked(lane, 2); }
 __device__ __forceinline__ unsigned cols_first_tile(int lane) { return lane * 16; }
 __host__ __device__ constexpr int tile_at(int row_tile, int column_tile) { return (row_tile * (row_tile + 1) / 2 + column_tile) * 512; }
@@ -126,7 +128,7 @@ struct DeltaSaved {
     float* rows;               // [slots, H, ROW_VALUES]
     __nv_bfloat16 *t, *t_rest; // [slots, H, MATRIX] blocked; t_rest only for an exact state
     __nv_bfloat16* p;
-    __nv_bfloat16 *states, *x; // S0 [slots, H, DV, D] blocked and X [slots, H, CHUNK, DV]; only for a backward
+    __nv_bfloat16 *states, *x; // S0 [slots, H, DV, D] and X, transposed, [slots, H, DV, CHUNK], both blocked; only for a backward
 };
 
 __device__ __forceinline__ float gate(const void* gates, int64_t index, bool is_bf16) {
@@ -214,6 +216,10 @@ cudaError_t launch_delta_chain(const DeltaShape& shape, const __nv_bfloat16* q, 
                                const float* initial, const DeltaSaved& saved, __nv_bfloat16* out, float* final_state,
                                cudaStream_t stream);
 cudaError_t launch_delta_backward(const DeltaShape& shape, const DeltaGradients& gradients, const DeltaSaved& saved, cudaStream_t stream);
+// The last stage of the backward on tcgen05, for D and DV of 64 or 128.
+cudaError_t launch_delta_gradient_tensor(const DeltaShape& shape, const DeltaGradients& gradients, const DeltaSaved& saved, cudaStream_t stream);
+// First bounded wait of the tensor-memory pipeline that ran out on the current device, 0 if none; reading clears it.
+cudaError_t read_delta_fault(int* code);
 cudaError_t launch_delta_step(const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v, const void* g, const void* beta,
                               bool gates_bf16, float scale, float* state, const int* slots, int64_t pool, int batch, int key_heads,
                               int heads, int d, int dv, __nv_bfloat16* out, cudaStream_t stream);

@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
                 }
             }
         const int count = min(CHUNK, length - c * CHUNK);
-        // the warp's 16 columns of the value tile are its own: X and O leave through them in rows of 32 bytes
+        // the warp's 16 columns of the value tile are its own: O leaves through them in rows of 32 bytes
         auto leave = [&](const float(&tiles)[TILES][4], char* to, int64_t stride, int rows_out) {
             __syncwarp();
 #pragma unroll
@@ -160,7 +160,11 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
                 if (t < rows_out) *reinterpret_cast<uint4*>(to + t * stride + (lane & 1) * 16) = piece;
             }
         };
-        if (SAVE) leave(x, reinterpret_cast<char*>(saved.x + place * CHUNK * dv + column), int64_t(dv) * 2, CHUNK);
+        if (SAVE) {
+            unsigned* to = reinterpret_cast<unsigned*>(saved.x + place * CHUNK * dv) + column / 8 * TILES * 32 + lane;
+#pragma unroll
+            for (int n = 0; n < TILES; ++n) to[n * 32] = pack2(x[n][0], x[n][1]), to[(TILES + n) * 32] = pack2(x[n][2], x[n][3]);
+        }
         // U, as left operand of P U; then with the decay to the chunk's end, of the state's update
         unsigned u[TILES / 2][4], u_rest[EXACT ? TILES / 2 : 1][4];
 #pragma unroll

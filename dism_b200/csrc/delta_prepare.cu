@@ -137,11 +137,13 @@ __global__ void __launch_bounds__(PREPARE_THREADS, 5) delta_prepare_kernel(Delta
             const double here = before + sum[e];
             const float hi = float(here), lo = float(here - double(hi));
             table[t] = hi, table[CHUNK + t] = lo, table[2 * CHUNK + t] = b[e];
-            rows[t] = ex2(hi) * (1.f + lo * .6931471805599453f);
-            rows[CHUNK + t] = b[e];
-            rows[2 * CHUNK + t] = ex2(float(total - here));
-            rows[3 * CHUNK + t] = hi;
-            rows[4 * CHUNK + t] = lo;
+            const float tail = ex2(float(total - here));
+            rows[ROW_DECAY + t] = ex2(hi) * (1.f + lo * .6931471805599453f);
+            rows[ROW_BETA + t] = b[e];
+            rows[ROW_TAIL + t] = tail;
+            rows[ROW_WRITE + t] = b[e] * tail;
+            rows[ROW_HIGH + t] = hi;
+            rows[ROW_LOW + t] = lo;
         }
     }
     cp_async_wait<0>();

@@ -1,0 +1,99 @@
+// Fifth-generation tensor cores for the delta rule kernels: bounded mbarrier waits, tensor memory, operand descriptors.
+//
+// Operand tiles in shared memory are blocks of rows of 128 bytes (64 bf16) with the 128-byte swizzle: piece p of row r lies at piece
+// p ^ (r & 7), a block starts at a multiple of 1024 bytes.  One and the same tile serves both ways round: with the contraction
+// along its rows (K-major; the next sixteen are 32 bytes further, the next eight rows 1024) and with the contraction across them
+// (MN-major; the next sixteen are 2048 bytes further, the next 64 of the other index one block further).
+#pragma once
+#include "dism_common.cuh"
+
+namespace dism {
+
+// Every wait is bounded, by about a second.  When one runs out, `abort` is set, the code is recorded and every later wait of the CTA
+// returns at once: all roles run to their ends with whatever the buffers hold, no product is issued any more, tensor memory is freed.
+constexpr unsigned TM_POLLS = 1u << 25;
+
+__device__ __forceinline__ uint32_t tm_address(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void tm_barrier_init(uint64_t* bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tm_address(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void tm_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tm_address(bar)) : "memory");
+}
+__device__ __forceinline__ bool tm_test(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{.reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}"
+                 : "=r"(done) : "r"(tm_address(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool tm_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort, int* fault, int code) {
+    for (unsigned polls = 0; polls < TM_POLLS; ++polls) {
+        if (tm_test(bar, parity)) return true;
+        if ((polls & 255) == 255 && *abort) return false;
+    }
+    *abort = 1;
+    atomicCAS(fault, 0, code);
+    return false;
+}
+// False: this wait ran out or another role's did.  Polling: these waits are links of a chain, and a parked warp wakes late.
+__device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* fault, int code) {
+    return tm_test(bar, parity) || tm_wait_slow(bar, parity, abort, fault, code);
+}
+
+__device__ __forceinline__ bool elect_one() {  // one lane of a converged warp
+    uint32_t elected;
+    asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(elected));
+    return elected != 0;
+}
+__device__ __forceinline__ void tm_allocate(uint32_t* to, uint32_t columns) {  // one whole warp
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tm_address(to)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tm_free(uint32_t at, uint32_t columns) {  // the same warp
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns) : "memory");
+}
+__device__ __forceinline__ void tm_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tm_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tm_fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tm_address(bar)) : "memory");
+}
+
+// Redistribution of a CTA's registers: every warp of four consecutive ones, counts from the launch's own share.
+template <int COUNT>
+__device__ __forceinline__ void tm_more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(COUNT)); }
+template <int COUNT>
+__device__ __forceinline__ void tm_fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(COUNT)); }
+
+// Lane = row, register i = column i; the warp's 32 lanes are rows 32 (warp % 4) .. of the tile.
+__device__ __forceinline__ void tm_load16(float (&v)[16], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+                   "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tm_store8(uint32_t at, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
+// Descriptors of swizzled tiles; `across` is the distance in bytes between blocks of 64 of the index that is not contracted (MN-major).
+__device__ __forceinline__ uint64_t tm_descriptor(uint32_t address, uint32_t across = 16) {
+    return uint64_t((address & 0x3ffff) >> 4) | (uint64_t(across >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+// bf16 x bf16 -> f32 with M = 128 rows and `columns` columns
+__host__ __device__ constexpr uint32_t tm_instruction(int columns, bool a_across, bool b_across) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (a_across ? 1u << 15 : 0u) | (b_across ? 1u << 16 : 0u) | (uint32_t(columns >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+}
+__device__ __forceinline__ void tm_mma_shared(uint32_t accumulator, uint64_t a, uint64_t b, uint32_t instruction, bool accumulate) {
+    asm volatile("{.reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}"
+                 ::"r"(accumulator), "l"(a), "l"(b), "r"(instruction), "r"(uint32_t(accumulate)) : "memory");
+}
+// The left operand in tensor memory: lane = row, a column holds two neighbouring bf16 of the contraction.
+__device__ __forceinline__ void tm_mma(uint32_t accumulator, uint32_t a, uint64_t b, uint32_t instruction, bool accumulate) {
+    asm volatile("{.reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}"
+                 ::"r"(accumulator), "r"(a), "l"(b), "r"(instruction), "r"(uint32_t(accumulate)) : "memory");
+}
+
+}  // namespace dism

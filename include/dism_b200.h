@@ -188,6 +188,10 @@ int dism_delta_backward(const void *q, const void *k, const void *dout, const fl
                         const void *saved, size_t saved_bytes, void *dq, void *dk, void *dv_out, void *dg, void *dbeta,
                         float *dinitial_state, void *workspace, size_t workspace_bytes, void *stream);
 
+/* The tensor-memory pipelines of the rule bound every wait; *code is the first that ran out on the current device since the last
+ * call (0: none, the only value a correct run produces); the call clears it.  Synchronises the device. */
+int dism_delta_fault(int *code);
+
 /* One token per row, state updated in place: q, k bf16 [batch,HK,D], v, out bf16 [batch,H,DV], g, beta [batch,H],
  * state float [pool,H,D,DV].  slots device int32 [batch]: the state of each row, or NULL for state i at row i.  A slot outside
  * [0, pool) marks a row without a sequence: its output is zero.  Rows that name one slot are taken in order, as consecutive

@@ -24,6 +24,17 @@ def flash():
     return flash_dism
 
 
+@pytest.fixture(autouse=True)
+def no_fault():
+    """No bounded wait of the tensor-memory pipelines runs out in any test."""
+    import ctypes
+    from dism_b200 import _lib
+    yield
+    code = ctypes.c_int(-1)
+    _lib.check(_lib.load().dism_delta_fault(ctypes.byref(code)))
+    assert code.value == 0
+
+
 def near(got, want, bound, heads_axis, what=''):
     got, want = (x.detach().double().cpu().movedim(heads_axis, 0).flatten(1) for x in (got, want))
     assert got.shape == want.shape and torch.isfinite(got).all(), what
