@@ -1,16 +1,19 @@
-// Gradients of one chunk of the gated delta rule on tcgen05 (D and DV of 64 or 128; delta_backward.cu has the other widths and the
-// formulas).  One CTA per chunk and key head walks the value heads that share the key head.
+// Gradients of the chunks of the gated delta rule on tcgen05 (D and DV of 64 or 128; delta_backward.cu has the other widths and the
+// formulas).  One CTA per SM walks (chunk, key head) units and, in each, the value heads that share the key head.
 //
 // Every product has M = 128: operands that meet the same right side are stacked.
 //     Z  = [dO; dY] X^T        QK = [Q; K] K^T        (128 x 64)
 //     U1 = [dO; dY] S0^T       U2 = [dP~; dL~] K      (128 x D)
-//     V1 = X dS1^T             V2 = dL~^T K + dP~^T Q  (64 x D; the rows stand twice, the left operand's other half being itself)
+//     V1 = X dS1^T             V2 = dL~^T K + dP~^T Q  (64 x D, in rows 64-127; what stands in the rows above is not read)
 // Rows 0-63 of Z, QK, U are the queries' part, rows 64-127 the keys', so a thread, which owns a row of tensor memory, forms
 //     dQ = scale e^G U1 + U2        or        dK = -e^G U1 + U2 + e^{G_63 - G} b V1 + V2
-// and all row sums of dG without a shuffle; column sums take one transposing reduction over the warp.  Each tile lies in shared
-// memory once and is read K-major or MN-major as a product needs it; [dP~; dL~] goes back there as bf16.
+// and all row sums of dG without a shuffle; column sums take one transposing reduction over the warp.  <dS1, S0> is the trace of one
+// more product.  Each tile lies in shared memory once and is read K-major or MN-major as a product needs it: Q, K, dO, dY and the
+// pairs [dP~; dL~] swizzled, X and the states in the 8 x 8 blocks in which they were kept, so that they arrive as three bulk copies.
 //
-// 192 KB in and 32 KB out of memory per chunk and head at D = DV = 128 against about 1200 clocks of tensor cores: the loads bound it.
+// What bounds it: 192 KB in and 32 KB out of memory per chunk and head at D = DV = 128, against about 1400 clocks of tensor cores.
+// All of Z, QK, U1, V1 and the trace are issued as soon as an item has landed; their end frees every tile but Q, K (of which there are
+// two) and the pairs, and the next item's loads run behind the rest of this one.
 #include "delta_common.cuh"
 #include "tensor_memory.cuh"
 
@@ -20,19 +23,21 @@ namespace {
 __device__ int delta_gradient_fault;
 
 constexpr int GRADIENT_THREADS = 256;
-constexpr uint32_t TM_Z = 0, TM_QK = 64, TM_U2 = 0, TM_U1 = 128, TM_V1 = 256, TM_V2 = 384, TM_COLUMNS = 512;  // U2 follows Z and QK
+// columns of tensor memory: U2 follows Z and QK, V2 the product whose trace is <dS1, S0>
+constexpr uint32_t TM_Z = 0, TM_QK = 64, TM_U2 = 0, TM_U1 = 128, TM_V1 = 256, TM_V2 = 384, TM_TRACE = 384, TM_COLUMNS = 512;
 
 template <int D, int DV>
 struct GradientTiles {
     static constexpr int STACK = 128 * 128;  // bytes of 128 rows by 64 columns
-    static constexpr int QK = 0, GRAD = QK + D / 64 * STACK, PAIRS = GRAD + DV / 64 * STACK, X = PAIRS + STACK, S0 = X + DV * 128, DS = S0 + 2 * D * DV;
-    static constexpr int ROWS = DS + 2 * D * DV, SUMS = ROWS + ROW_VALUES * 4;
-    // floats: rows of M [2][128], its columns [4][64], columns of b [2][64], state terms of dG [2][128], of dG_63 [2][64], <dS1, S0> [8]
-    static constexpr int ROW_SUM = 0, COLUMN_SUM = 256, BETA_SUM = COLUMN_SUM + 256, STATE_SUM = BETA_SUM + 128, LAST_SUM = STATE_SUM + 256, DOT = LAST_SUM + 128;
-    static constexpr int BYTES = SUMS + (DOT + 8) * 4 + 1024;  // and room to start at a multiple of 1024
+    static constexpr int STATE = 2 * D * DV;
+    static constexpr int QK = 0, GRAD = QK + 2 * (D / 64) * STACK, PAIRS = GRAD + DV / 64 * STACK, X = PAIRS + STACK, S0 = X + DV * 128, DS = S0 + STATE;
+    static constexpr int ROWS = DS + STATE, SUMS = ROWS + 2 * ROW_VALUES * 4;
+    // floats: rows of M [2][128], columns of M / b [4][64], state terms of dG [2][128], of dG_63 [2][64], <dS1, S0> [4], the part of db from dU [64]
+    static constexpr int ROW_SUM = 0, COLUMN_SUM = 256, STATE_SUM = COLUMN_SUM + 256, LAST_SUM = STATE_SUM + 256, DOT = LAST_SUM + 128, BETA = DOT + 4;
+    static constexpr int BYTES = SUMS + (BETA + 64) * 4 + 1024;  // and room to start at a multiple of 1024
 };
 struct GradientControl {
-    uint64_t first, second;
+    uint64_t loaded, first, second;
     uint32_t tensor_memory;
     int abort;
 };
@@ -50,16 +55,6 @@ __device__ __forceinline__ void load_stack(unsigned tile, const char* global, in
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + row * 128 + (((piece & 7) ^ ((first + row) & 7)) * 16)),
                      "l"(inside ? from : global), "r"(inside ? 16 : 0) : "memory");
         from += STEP * stride;
-    }
-}
-// ROWS x WIDTH elements kept as 8 x 8 blocks into swizzled blocks of 64 columns
-template <int ROWS, int WIDTH>
-__device__ __forceinline__ void load_blocked(unsigned tile, const __nv_bfloat16* global, int thread) {
-#pragma unroll
-    for (int i = thread; i < ROWS * WIDTH / 8; i += GRADIENT_THREADS) {
-        const int block = i >> 3, r = i & 7, column = block % (WIDTH / 8), row = block / (WIDTH / 8) * 8 + r;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tile + (column >> 3) * (ROWS * 128) + row * 128 + (((column & 7) ^ r) * 16)),
-                     "l"(global + i * 8) : "memory");
     }
 }
 // v[i] of every lane is summed over the warp for each i; lane l keeps the sum of i = l
@@ -88,102 +83,117 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
     extern __shared__ unsigned char shared_raw[];
     unsigned char* shared = shared_raw + ((1024 - (tm_address(shared_raw) & 1023)) & 1023);
     __shared__ GradientControl control;
-    const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31, key_head = blockIdx.y, group = shape.heads / shape.key_heads;
-    int64_t row;
-    int count;
-    const int64_t slot = blockIdx.x;
-    shape.layout.chunk(slot, row, count);
-    if (count == 0) return;
+    const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31, group = shape.heads / shape.key_heads;
+    const int64_t units = shape.layout.slots() * shape.key_heads;
+    int64_t row = 0, next_row = 0, unit = blockIdx.x, next_unit;
+    int count = 0, next_count = 0;
+    // the first unit from `from` on that has positions
+    auto find = [&](int64_t from, int64_t& at, int& positions) {
+        for (; from < units; from += gridDim.x) {
+            shape.layout.chunk(from / shape.key_heads, at, positions);
+            if (positions > 0) break;
+        }
+        return from;
+    };
+    unit = find(unit, row, count);
+    if (unit >= units) return;
     const uint32_t base = tm_address(shared);
-    const float* rows = reinterpret_cast<const float*>(shared + Tiles::ROWS);
     float* sums = reinterpret_cast<float*>(shared + Tiles::SUMS);
     const int64_t key_stride = int64_t(shape.key_heads) * D * 2, value_stride = int64_t(shape.heads) * DV * 2;
-    const int64_t key = (row * shape.key_heads + key_head) * D * 2;
-    load_stack<D, STACK>(base + Tiles::QK, reinterpret_cast<const char*>(q) + key, key_stride, count, thread);
-    load_stack<D, STACK>(base + Tiles::QK + HALF, reinterpret_cast<const char*>(k) + key, key_stride, count, thread);
     if (thread == 0) {
-        tm_barrier_init(&control.first, 1), tm_barrier_init(&control.second, 1);
+        tm_barrier_init(&control.loaded, 1), tm_barrier_init(&control.first, 1), tm_barrier_init(&control.second, 1);
         control.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) tm_allocate(&control.tensor_memory, TM_COLUMNS);
+    tm_fence_before();
+    __syncthreads();
+    tm_fence_after();
     volatile int* abort = &control.abort;
-    uint32_t tensor = 0;
+    const uint32_t tensor = control.tensor_memory, lanes = tensor + (uint32_t((warp & 3) * 32) << 16);
+
+    // an item's loads; `item` counts the CTA's items, `keys` is the buffer of Q and K, filled for the first head of a unit
+    auto load = [&](int64_t of_unit, int64_t at, int positions, int turn, int item, int keys) {
+        const int key_head = int(of_unit % shape.key_heads), head = key_head * group + turn;
+        const int64_t place = of_unit / shape.key_heads * shape.heads + head;
+        if (thread == 0) {
+            tm_expect(&control.loaded, DV * 128 + 2 * Tiles::STATE);
+            tm_copy(base + Tiles::X, saved.x + place * CHUNK * DV, DV * 128, &control.loaded);
+            tm_copy(base + Tiles::S0, saved.states + place * D * DV, Tiles::STATE, &control.loaded);
+            tm_copy(base + Tiles::DS, dstates + place * D * DV, Tiles::STATE, &control.loaded);
+        }
+        const int64_t value = (at * shape.heads + head) * DV * 2;
+        load_stack<DV, STACK>(base + Tiles::GRAD, reinterpret_cast<const char*>(dout) + value, value_stride, positions, thread);
+        load_stack<DV, STACK>(base + Tiles::GRAD + HALF, reinterpret_cast<const char*>(dy) + value, value_stride, positions, thread);
+        load_block<ROW_VALUES * 4, GRADIENT_THREADS>(base + Tiles::ROWS + (item & 1) * ROW_VALUES * 4, reinterpret_cast<const char*>(saved.rows + place * ROW_VALUES), thread);
+        if (turn == 0) {
+            const int64_t key = (at * shape.key_heads + key_head) * D * 2;
+            const uint32_t to = base + Tiles::QK + keys * (D / 64 * STACK);
+            load_stack<D, STACK>(to, reinterpret_cast<const char*>(q) + key, key_stride, positions, thread);
+            load_stack<D, STACK>(to + HALF, reinterpret_cast<const char*>(k) + key, key_stride, positions, thread);
+        }
+        cp_async_commit();
+    };
 
     // this thread's row of tensor memory: position t, a query's (part 0) or a key's (part 1); its half of the columns
     const int r = thread & 127, t = r & 63, part = r >> 6, half = warp >> 2;
     float acc[COLUMNS];  // half a row of dQ or dK
 #pragma unroll
     for (int i = 0; i < COLUMNS; ++i) acc[i] = 0.f;
-
-    for (int turn = 0; turn < group; ++turn) {
-        const int head = key_head * group + turn;
-        const int64_t place = slot * shape.heads + head;
-        const int64_t value = (row * shape.heads + head) * DV * 2;
-        load_stack<DV, STACK>(base + Tiles::GRAD, reinterpret_cast<const char*>(dout) + value, value_stride, count, thread);
-        load_stack<DV, STACK>(base + Tiles::GRAD + HALF, reinterpret_cast<const char*>(dy) + value, value_stride, count, thread);
-        load_blocked<DV, CHUNK>(base + Tiles::X, saved.x + place * CHUNK * DV, thread);
-        load_block<ROW_VALUES * 4, GRADIENT_THREADS>(base + Tiles::ROWS, reinterpret_cast<const char*>(saved.rows + place * ROW_VALUES), thread);
-        cp_async_commit();
-        load_blocked<DV, D>(base + Tiles::S0, saved.states + place * D * DV, thread);
-        load_blocked<DV, D>(base + Tiles::DS, dstates + place * D * DV, thread);
-        cp_async_commit();
-        cp_async_wait<1>();
-        tm_fence_proxy();
-        tm_fence_before();
+    load(unit, row, count, 0, 0, 0);
+    for (int item = 0, turn = 0, keys = 0;; ++item) {
+        const int key_head = int(unit % shape.key_heads), head = key_head * group + turn;
+        const int64_t place = unit / shape.key_heads * shape.heads + head;
+        const uint32_t parity = item & 1, qk_tile = base + Tiles::QK + keys * (D / 64 * STACK);
+        const float* rows = reinterpret_cast<const float*>(shared + Tiles::ROWS + (item & 1) * ROW_VALUES * 4);
+        cp_async_wait<0>();
+        tm_fence_proxy();  // written through the generic proxy, read by the tensor cores
+        tm_wait(&control.loaded, parity, abort, &delta_gradient_fault, 3);
         __syncthreads();
         tm_fence_after();
-        tensor = control.tensor_memory;
-        const uint32_t lanes = tensor + (uint32_t((warp & 3) * 32) << 16);
-        const uint64_t grads = tm_descriptor(base + Tiles::GRAD), keys_across = tm_descriptor(base + Tiles::QK + HALF, STACK);
+        const uint64_t keys_across = tm_descriptor(qk_tile + HALF, STACK);
         if (warp == 0 && !*abort) {
             if (elect_one()) {
-                const uint64_t x = tm_descriptor(base + Tiles::X), qk = tm_descriptor(base + Tiles::QK), keys = tm_descriptor(base + Tiles::QK + HALF);
+                const uint64_t grads = tm_descriptor(base + Tiles::GRAD), x = tm_block_descriptor(base + Tiles::X, 128, CHUNK * 16);
+                const uint64_t queries = tm_descriptor(qk_tile), own_keys = tm_descriptor(qk_tile + HALF);
+                const uint64_t s0 = tm_block_descriptor(base + Tiles::S0, 128, D * 16), ds = tm_block_descriptor(base + Tiles::DS, 128, D * 16);
 #pragma unroll
                 for (int kb = 0; kb < DV / 16; ++kb)
-                    tm_mma_shared(tensor + TM_Z, grads + ((kb >> 2) * STACK + (kb & 3) * 32) / 16, x + kb * 2048 / 16, tm_instruction(CHUNK, false, true), kb > 0);
+                    tm_mma_shared(tensor + TM_Z, grads + ((kb >> 2) * STACK + (kb & 3) * 32) / 16, x + kb * CHUNK * 2, tm_instruction(CHUNK, false, true), kb > 0);
 #pragma unroll
                 for (int kb = 0; kb < D / 16; ++kb)
-                    tm_mma_shared(tensor + TM_QK, qk + ((kb >> 2) * STACK + (kb & 3) * 32) / 16, keys + ((kb >> 2) * STACK + (kb & 3) * 32) / 16,
+                    tm_mma_shared(tensor + TM_QK, queries + ((kb >> 2) * STACK + (kb & 3) * 32) / 16, own_keys + ((kb >> 2) * STACK + (kb & 3) * 32) / 16,
                                   tm_instruction(CHUNK, false, false), kb > 0);
+#pragma unroll
+                for (int kb = 0; kb < DV / 16; ++kb)
+                    tm_mma_shared(tensor + TM_U1, grads + ((kb >> 2) * STACK + (kb & 3) * 32) / 16, s0 + kb * D * 2, tm_instruction(D, false, true), kb > 0);
+                // X as rows 64-127: eight blocks before it begins
+#pragma unroll
+                for (int kb = 0; kb < DV / 16; ++kb)
+                    tm_mma_shared(tensor + TM_V1, x - 1024 / 16 + kb * CHUNK * 2, ds + kb * D * 2, tm_instruction(D, true, true), kb > 0);
+#pragma unroll
+                for (int kb = 0; kb < DV / 16; ++kb)
+                    tm_mma_shared(tensor + TM_TRACE, s0 + kb * D * 2, ds + kb * D * 2, tm_instruction(D, true, true), kb > 0);
                 tm_commit(&control.first);
             }
             __syncwarp();
         }
-        cp_async_wait<0>();
-        tm_fence_proxy();
-        __syncthreads();
-        if (warp == 0 && !*abort) {
-            if (elect_one()) {
-                const uint64_t s0 = tm_descriptor(base + Tiles::S0, DV * 128), ds = tm_descriptor(base + Tiles::DS, DV * 128), x = tm_descriptor(base + Tiles::X, 0);
+        float beta_part = 0.f;  // what the reverse chain left of db
+        if (thread < CHUNK) {
+            const int64_t stride = shape.layout.slots() * shape.heads * CHUNK;
 #pragma unroll
-                for (int kb = 0; kb < DV / 16; ++kb)
-                    tm_mma_shared(tensor + TM_U1, grads + ((kb >> 2) * STACK + (kb & 3) * 32) / 16, s0 + kb * 2048 / 16, tm_instruction(D, false, true), kb > 0);
-#pragma unroll
-                for (int kb = 0; kb < DV / 16; ++kb)
-                    tm_mma_shared(tensor + TM_V1, x + kb * 2048 / 16, ds + kb * 2048 / 16, tm_instruction(D, true, true), kb > 0);
-            }
-            __syncwarp();
+            for (int i = 0; i < DV / 16; ++i) beta_part += __ldg(dbeta_parts + i * stride + place * CHUNK + thread);
         }
-        {
-            float dot = 0.f;  // <dS1, S0>
-            const uint4 *s0 = reinterpret_cast<const uint4*>(shared + Tiles::S0), *ds = reinterpret_cast<const uint4*>(shared + Tiles::DS);
-#pragma unroll 4
-            for (int i = thread; i < D * DV / 8; i += GRADIENT_THREADS) {
-                const uint4 x = s0[i], y = ds[i];
-                dot += low_half(x.x) * low_half(y.x) + high_half(x.x) * high_half(y.x) + low_half(x.y) * low_half(y.y) + high_half(x.y) * high_half(y.y);
-                dot += low_half(x.z) * low_half(y.z) + high_half(x.z) * high_half(y.z) + low_half(x.w) * low_half(y.w) + high_half(x.w) * high_half(y.w);
-            }
-#pragma unroll
-            for (int m = 16; m; m >>= 1) dot += __shfl_xor_sync(FULL, dot, m);
-            if (lane == 0) sums[Tiles::DOT + warp] = dot;
-        }
-        // dP~ or dL~ of this row: columns 32 half .. 32 half + 31
-        tm_wait(&control.first, turn & 1, abort, &delta_gradient_fault, 1);
+        const bool same_unit = turn + 1 < group;
+        next_unit = same_unit ? unit : find(unit + gridDim.x, next_row, next_count);
+        if (same_unit) next_row = row, next_count = count;
+        tm_wait(&control.first, parity, abort, &delta_gradient_fault, 1);
         tm_fence_after();
+        if (next_unit < units) load(next_unit, next_row, next_count, same_unit ? turn + 1 : 0, item + 1, same_unit ? keys : keys ^ 1);
+        // dP~ or dL~ of this row: columns 32 half .. 32 half + 31
         {
             const float high = rows[ROW_HIGH + t], low = rows[ROW_LOW + t];
-            float m[32], w[32], row_sum = 0.f;
+            float w[32], row_sum = 0.f;
 #pragma unroll
             for (int j = 0; j < 32; j += 16) {
                 float z[16], y[16];
@@ -199,8 +209,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                     const float x = counts ? (part ? -between : shape.scale * between) * z[i] : 0.f;
                     d[i] = x * rows[ROW_BETA + s];
                     w[j + i] = x * y[i];
-                    m[j + i] = d[i] * y[i];
-                    row_sum += m[j + i];
+                    row_sum += __fmul_rn(rows[ROW_BETA + s], w[j + i]);  // as the column sums have it: a pair that cancels in dG is one number
                 }
 #pragma unroll
                 for (int i = 0; i < 16; i += 8)
@@ -208,8 +217,22 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                         make_uint4(pack2(d[i], d[i + 1]), pack2(d[i + 2], d[i + 3]), pack2(d[i + 4], d[i + 5]), pack2(d[i + 6], d[i + 7]));
             }
             sums[Tiles::ROW_SUM + half * 128 + r] = row_sum;
-            sums[Tiles::COLUMN_SUM + (warp & 3) * CHUNK + 32 * half + lane] = transposing_sum(m, lane);
-            if (part) sums[Tiles::BETA_SUM + (warp & 1) * CHUNK + 32 * half + lane] = transposing_sum(w, lane);
+            sums[Tiles::COLUMN_SUM + (warp & 3) * CHUNK + 32 * half + lane] = transposing_sum(w, lane);
+            if (half == 0 && r < D) {  // the trace: element r of this row
+                float dot = 0.f;
+#pragma unroll
+                for (int j = 0; j < 32; j += 16) {
+                    float x[16];
+                    tm_load16(x, lanes + TM_TRACE + (warp & 3) * 32 + j);
+                    tm_wait_load();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) dot += j + i == lane ? x[i] : 0.f;
+                }
+#pragma unroll
+                for (int m = 16; m; m >>= 1) dot += __shfl_xor_sync(FULL, dot, m);
+                if (lane == 0) sums[Tiles::DOT + warp] = dot;
+            }
+            if (thread < CHUNK) sums[Tiles::BETA + thread] = beta_part;
         }
         tm_fence_proxy();
         tm_fence_before();
@@ -218,7 +241,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
         if (warp == 0 && !*abort) {
             if (elect_one()) {
                 const uint64_t pairs = tm_descriptor(base + Tiles::PAIRS), p_across = tm_descriptor(base + Tiles::PAIRS, 0), l_across = tm_descriptor(base + Tiles::PAIRS + HALF, 0);
-                const uint64_t queries_across = tm_descriptor(base + Tiles::QK, STACK);
+                const uint64_t queries_across = tm_descriptor(qk_tile, STACK);
 #pragma unroll
                 for (int kb = 0; kb < CHUNK / 16; ++kb)
                     tm_mma_shared(tensor + TM_U2, pairs + kb * 32 / 16, keys_across + kb * 2048 / 16, tm_instruction(D, false, true), kb > 0);
@@ -232,12 +255,12 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
             }
             __syncwarp();
         }
-        tm_wait(&control.second, turn & 1, abort, &delta_gradient_fault, 2);
+        tm_wait(&control.second, parity, abort, &delta_gradient_fault, 2);
         tm_fence_after();
         {
             const float decay = rows[ROW_DECAY + t], f1 = part ? -decay : shape.scale * decay, f2 = rows[ROW_WRITE + t];
             float state_sum = 0.f, last_sum = 0.f;
-            const unsigned char* own = shared + Tiles::QK + (half * COLUMNS >> 6) * STACK + r * 128;  // the row of Q or K
+            const unsigned char* own = shared + Tiles::QK + keys * (D / 64 * STACK) + (half * COLUMNS >> 6) * STACK + r * 128;  // the row of Q or K
 #pragma unroll
             for (int j = 0; j < COLUMNS; j += 16) {
                 const int column = half * COLUMNS + j;
@@ -275,18 +298,15 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int p = 2 * lane + e;
-                const float tail = sums[Tiles::LAST_SUM + p] + sums[Tiles::LAST_SUM + CHUNK + p];
+                const float tail = sums[Tiles::LAST_SUM + p] + sums[Tiles::LAST_SUM + CHUNK + p], beta = rows[ROW_BETA + p];
                 float x = 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    x += (sums[Tiles::ROW_SUM + i * CHUNK + p] - sums[Tiles::COLUMN_SUM + i * CHUNK + p]) + sums[Tiles::STATE_SUM + i * CHUNK + p];
+                    x += (sums[Tiles::ROW_SUM + i * CHUNK + p] - __fmul_rn(beta, sums[Tiles::COLUMN_SUM + i * CHUNK + p])) + sums[Tiles::STATE_SUM + i * CHUNK + p];
                 here[e] = x - tail;
                 last += tail;
-                float b = sums[Tiles::BETA_SUM + p] + sums[Tiles::BETA_SUM + CHUNK + p];
-                const int64_t stride = shape.layout.slots() * shape.heads * CHUNK;
-#pragma unroll
-                for (int i = 0; i < DV / 16; ++i) b += __ldg(dbeta_parts + i * stride + place * CHUNK + p);
                 if (p < count) {
+                    const float b = sums[Tiles::BETA + p] + (sums[Tiles::COLUMN_SUM + 2 * CHUNK + p] + sums[Tiles::COLUMN_SUM + 3 * CHUNK + p]);
                     const int64_t index = (row + p) * shape.heads + head;
                     if (shape.gates_bf16) static_cast<__nv_bfloat16*>(dbeta)[index] = __float2bfloat16(b);
                     else static_cast<float*>(dbeta)[index] = b;
@@ -296,7 +316,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
             for (int m = 16; m; m >>= 1) last += __shfl_xor_sync(FULL, last, m);
             float dot = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dot += sums[Tiles::DOT + i];
+            for (int i = 0; i < D / 32; ++i) dot += sums[Tiles::DOT + i];
             last += rows[ROW_DECAY + CHUNK - 1] * dot;
             if (lane == 31) here[1] += last;
             here[0] += here[1];
@@ -321,16 +341,23 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                 }
             }
         }
-        if (turn + 1 < group) __syncthreads();  // tiles and sums are free for the next head
-    }
-    if (t < count) {
-        __nv_bfloat16* to = (part ? dk : dq) + ((row + t) * shape.key_heads + key_head) * D + half * COLUMNS;
+        if (!same_unit) {
+            if (t < count) {
+                __nv_bfloat16* to = (part ? dk : dq) + ((row + t) * shape.key_heads + key_head) * D + half * COLUMNS;
 #pragma unroll
-        for (int i = 0; i < COLUMNS; i += 8)
-            *reinterpret_cast<uint4*>(to + i) = make_uint4(pack2(acc[i], acc[i + 1]), pack2(acc[i + 2], acc[i + 3]), pack2(acc[i + 4], acc[i + 5]), pack2(acc[i + 6], acc[i + 7]));
+                for (int i = 0; i < COLUMNS; i += 8)
+                    *reinterpret_cast<uint4*>(to + i) = make_uint4(pack2(acc[i], acc[i + 1]), pack2(acc[i + 2], acc[i + 3]), pack2(acc[i + 4], acc[i + 5]), pack2(acc[i + 6], acc[i + 7]));
+            }
+            if (next_unit >= units) break;
+#pragma unroll
+            for (int i = 0; i < COLUMNS; ++i) acc[i] = 0.f;
+            keys ^= 1;
+        }
+        turn = same_unit ? turn + 1 : 0;
+        unit = next_unit, row = next_row, count = next_count;
     }
     __syncthreads();
-    if (control.abort) __nanosleep(1000000);  // products in flight end before their memory is given back
+    if (control.abort) __nanosleep(1000000);  // copies and products in flight end before their memory is given back
     if (warp == 0) {
         tm_fence_after();
         tm_free(tensor, TM_COLUMNS);
@@ -343,7 +370,8 @@ cudaError_t launch(const DeltaShape& shape, const DeltaGradients& x, const Delta
     auto* kernel = delta_gradient_tensor_kernel<D, DV>;
     if (cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES)) return status;
     KernelTimer timer("delta_gradient", stream);
-    kernel<<<dim3(unsigned(shape.layout.slots()), shape.key_heads), GRADIENT_THREADS, BYTES, stream>>>(
+    const int64_t units = shape.layout.slots() * shape.key_heads;
+    kernel<<<unsigned(units < device_sm_count() ? units : device_sm_count()), GRADIENT_THREADS, BYTES, stream>>>(
         shape, x.q, x.k, x.dout, x.dv, saved, x.dstates, x.dbeta_parts, x.dq, x.dk, x.dg, x.dbeta);
     return cudaGetLastError();
 }

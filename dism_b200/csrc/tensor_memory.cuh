@@ -40,6 +40,14 @@ __device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, volatile
     return tm_test(bar, parity) || tm_wait_slow(bar, parity, abort, fault, code);
 }
 
+// Contiguous bytes (a multiple of 16, both addresses 16-byte aligned) into shared memory; the barrier counts them.
+__device__ __forceinline__ void tm_expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tm_address(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tm_copy(uint32_t to, const void* from, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(to), "l"(from), "r"(bytes), "r"(tm_address(bar)) : "memory");
+}
 __device__ __forceinline__ bool elect_one() {  // one lane of a converged warp
     uint32_t elected;
     asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(elected));
@@ -81,6 +89,11 @@ __device__ __forceinline__ void tm_store8(uint32_t at, const uint32_t (&v)[8]) {
 // Descriptors of swizzled tiles; `across` is the distance in bytes between blocks of 64 of the index that is not contracted (MN-major).
 __device__ __forceinline__ uint64_t tm_descriptor(uint32_t address, uint32_t across = 16) {
     return uint64_t((address & 0x3ffff) >> 4) | (uint64_t(across >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+// The same for tiles of 8 x 8 blocks of 128 contiguous bytes, a block's rows along the contraction (MN-major, no swizzle): distances
+// between blocks along the other index and along the contraction.
+__device__ __forceinline__ uint64_t tm_block_descriptor(uint32_t address, uint32_t other, uint32_t contracted) {
+    return uint64_t((address & 0x3ffff) >> 4) | (uint64_t(contracted >> 4) << 16) | (uint64_t(other >> 4) << 32) | (uint64_t(1) << 46);
 }
 // bf16 x bf16 -> f32 with M = 128 rows and `columns` columns
 __host__ __device__ constexpr uint32_t tm_instruction(int columns, bool a_across, bool b_across) {
