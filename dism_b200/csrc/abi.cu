@@ -314,7 +314,7 @@ static int check_delta(int packed, int sequences, int n, int key_heads, int head
 namespace {
 constexpr size_t round_up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 // The parts of `saved`, in the order in which they lie; those that `exact` or `backward` do not ask for have no bytes.
-size_t lay_out_delta(const dism::DeltaShape& shape, bool exact, bool backward, char* base, dism::DeltaSaved* saved) {
+size_t lay_out_delta(dism::DeltaShape& shape, bool exact, bool backward, char* base, dism::DeltaSaved* saved) {
     const size_t places = size_t(shape.layout.slots()) * shape.heads;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -331,33 +331,40 @@ size_t lay_out_delta(const dism::DeltaShape& shape, bool exact, bool backward, c
         parts.states = reinterpret_cast<bf*>(take(places * shape.d * shape.dv * 2));
         parts.x = reinterpret_cast<bf*>(take(places * dism::CHUNK * shape.dv * 2));
     }
+    const size_t segments = shape.segments.length ? size_t(shape.segments.count(shape.layout)) * shape.heads : 0;
+    shape.segments.m = reinterpret_cast<bf*>(take(segments * shape.d * shape.d * 2));
+    if (exact) shape.segments.m_rest = reinterpret_cast<bf*>(take(segments * shape.d * shape.d * 2));
+    shape.segments.ends = reinterpret_cast<float*>(take(segments * shape.d * shape.dv * 4));
     if (exact) parts.t_rest = reinterpret_cast<bf*>(take(places * dism::MATRIX * 2));
     if (saved) *saved = parts;
     return at;
 }
 size_t delta_scratch(const dism::DeltaShape& shape, char* base, dism::DeltaGradients* x) {
     const size_t places = size_t(shape.layout.slots()) * shape.heads;
-    const size_t states = round_up(places * shape.d * shape.dv * 2);
+    const size_t segments = shape.segments.length ? size_t(shape.segments.count(shape.layout)) * shape.heads : 0;
+    const size_t states = round_up(places * shape.d * shape.dv * 2), parts = round_up(places * dism::CHUNK * (shape.dv / 16) * 4);
     if (x) {
         x->dstates = reinterpret_cast<__nv_bfloat16*>(base);
         x->dbeta_parts = reinterpret_cast<float*>(base + states);
+        x->ends = reinterpret_cast<float*>(base + states + parts);
     }
-    return states + round_up(places * dism::CHUNK * (shape.dv / 16) * 4);
+    return states + parts + round_up(segments * shape.d * shape.dv * 4);
 }
 dism::DeltaShape delta_shape(const int32_t* cu_seqlens, int sequences, int n, int key_heads, int heads, int d, int dv, int gates_bf16, float scale) {
-    return dism::DeltaShape{dism::DeltaLayout{cu_seqlens, sequences, n}, key_heads, heads, d, dv, gates_bf16 != 0, scale};
+    const dism::DeltaLayout layout{cu_seqlens, sequences, n};
+    return dism::DeltaShape{layout, dism::DeltaSegments{dism::delta_segment_length(layout, heads, d, dv), nullptr, nullptr, nullptr}, key_heads, heads, d, dv, gates_bf16 != 0, scale};
 }
 }  // namespace
 
 size_t dism_delta_saved(int packed, int sequences, int n, int heads, int d, int dv, int final_state, int backward) {
     if (check_delta(packed, sequences, n, 1, heads, d, dv)) return 0;
-    const auto shape = delta_shape(packed ? reinterpret_cast<const int32_t*>(4) : nullptr, sequences, n, 1, heads, d, dv, 0, 1.f);
+    auto shape = delta_shape(packed ? reinterpret_cast<const int32_t*>(4) : nullptr, sequences, n, 1, heads, d, dv, 0, 1.f);
     return lay_out_delta(shape, final_state != 0, backward != 0, nullptr, nullptr);
 }
 
 size_t dism_delta_backward_workspace(int packed, int sequences, int n, int heads, int d, int dv) {
     if (check_delta(packed, sequences, n, 1, heads, d, dv)) return 0;
-    const auto shape = delta_shape(packed ? reinterpret_cast<const int32_t*>(4) : nullptr, sequences, n, 1, heads, d, dv, 0, 1.f);
+    auto shape = delta_shape(packed ? reinterpret_cast<const int32_t*>(4) : nullptr, sequences, n, 1, heads, d, dv, 0, 1.f);
     return delta_scratch(shape, nullptr, nullptr);
 }
 
@@ -369,7 +376,7 @@ int dism_delta_forward(const void* q, const void* k, const void* v, const void* 
     if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16)) return fail(DISM_EINVAL, "vector tensors must be 16-byte aligned");
     if (!aligned(initial_state, 16) || !aligned(final_state, 16) || !aligned(g, gates_bf16 ? 2 : 4) || !aligned(beta, gates_bf16 ? 2 : 4) || !aligned(cu_seqlens, 4))
         return fail(DISM_EINVAL, "states must be 16-byte aligned, gates and sequence starts to their size");
-    const auto shape = delta_shape(cu_seqlens, sequences, n, key_heads, heads, d, dv, gates_bf16, scale);
+    auto shape = delta_shape(cu_seqlens, sequences, n, key_heads, heads, d, dv, gates_bf16, scale);
     dism::DeltaSaved parts;
     if (!saved || !aligned(saved, 256) || saved_bytes < lay_out_delta(shape, final_state != nullptr, backward != 0, static_cast<char*>(saved), &parts))
         return fail(DISM_EINVAL, "workspace missing, too small or misaligned (see dism_delta_saved)");
@@ -390,12 +397,12 @@ int dism_delta_backward(const void* q, const void* k, const void* dout, const fl
         return fail(DISM_EINVAL, "vector tensors must be 16-byte aligned");
     if (!aligned(dfinal_state, 16) || !aligned(dinitial_state, 16) || !aligned(dg, gates_bf16 ? 2 : 4) || !aligned(dbeta, gates_bf16 ? 2 : 4) || !aligned(cu_seqlens, 4))
         return fail(DISM_EINVAL, "states must be 16-byte aligned, gates and sequence starts to their size");
-    const auto shape = delta_shape(cu_seqlens, sequences, n, key_heads, heads, d, dv, gates_bf16, scale);
+    auto shape = delta_shape(cu_seqlens, sequences, n, key_heads, heads, d, dv, gates_bf16, scale);
     dism::DeltaSaved parts;
     if (!saved || !aligned(saved, 256) || saved_bytes < lay_out_delta(shape, false, true, const_cast<char*>(static_cast<const char*>(saved)), &parts))
         return fail(DISM_EINVAL, "saved buffer missing, too small or misaligned (see dism_delta_saved)");
     using bf = __nv_bfloat16;
-    dism::DeltaGradients x{static_cast<const bf*>(q), static_cast<const bf*>(k), static_cast<const bf*>(dout), dfinal_state, nullptr, nullptr,
+    dism::DeltaGradients x{static_cast<const bf*>(q), static_cast<const bf*>(k), static_cast<const bf*>(dout), dfinal_state, nullptr, nullptr, nullptr,
                            static_cast<bf*>(dq), static_cast<bf*>(dk), static_cast<bf*>(dv_out), dg, dbeta, dinitial_state};
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < delta_scratch(shape, static_cast<char*>(workspace), &x))
         return fail(DISM_EINVAL, "workspace missing, too small or misaligned (see dism_delta_backward_workspace)");

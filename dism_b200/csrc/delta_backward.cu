@@ -25,23 +25,39 @@ struct ReverseStage {
     static constexpr int X = 2 * BYTES, TOTAL = X + CHUNK * VALUE_PITCH;  // one X for both stages: its columns belong to a warp each
 };
 
-template <int D, int WARPS>
+// LOCAL: the first launch over segments: from a zero gradient behind the segment to the one before it, no outputs.
+template <int D, int WARPS, bool LOCAL>
 __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape shape, const __nv_bfloat16* __restrict__ q,
                                                                    const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ dout,
                                                                    const float* __restrict__ dfinal, DeltaSaved saved,
                                                                    __nv_bfloat16* __restrict__ dstates, float* __restrict__ dbeta_parts,
-                                                                   __nv_bfloat16* __restrict__ dv_out, float* __restrict__ dinitial) {
+                                                                   __nv_bfloat16* __restrict__ dv_out, float* __restrict__ dinitial, float* __restrict__ ends) {
     using Stage = ReverseStage<D, WARPS>;
     constexpr int THREADS = WARPS * 32, TILES = CHUNK / 8;
     extern __shared__ __align__(128) unsigned char shared[];
     const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
-    const int head = blockIdx.y, sequence = blockIdx.x, dv = shape.dv;
+    const int head = blockIdx.y, dv = shape.dv;
     const int key_head = head / (shape.heads / shape.key_heads), column = (blockIdx.z * WARPS + warp) * 16;
     int64_t row, slot;
-    int length;
+    int length, sequence, number;
+    shape.segments.find(shape.layout, blockIdx.x, sequence, number);
     shape.layout.span(sequence, row, length, slot);
-    const int chunks = (length + CHUNK - 1) / CHUNK;
     const unsigned base = smem_address(shared);
+    if (!LOCAL && shape.layout.cu && number == 0) {
+        char* to = reinterpret_cast<char*>(dv_out + int64_t(head) * dv + blockIdx.z * WARPS * 16);
+        const int64_t stride = int64_t(shape.heads) * dv * 2;
+        if (sequence == 0) clear_rows<WARPS * 32>(to, stride, WARPS * 2, 0, row, thread);
+        if (sequence == shape.layout.sequences - 1) clear_rows<WARPS * 32>(to, stride, WARPS * 2, row + length, shape.layout.n, thread);
+    }
+    int chunks = (length + CHUNK - 1) / CHUNK, behind = 0;  // segments behind this one
+    if (shape.segments.length) {
+        const int before = min(number * shape.segments.length, chunks);
+        if (number && before == chunks) return;  // no such segment
+        if (LOCAL && number == 0) return;
+        behind = (chunks - 1 - before) / shape.segments.length;
+        chunks = min(chunks - before, shape.segments.length);
+        slot += before, row += int64_t(before) * CHUNK, length -= before * CHUNK;
+    }
     const int64_t key_stride = int64_t(shape.key_heads) * D * 2, value_stride = int64_t(shape.heads) * dv * 2;
     auto load = [&](int c) {
         const unsigned stage = base + (c & 1) * Stage::BYTES;
@@ -65,12 +81,45 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
     for (int n = 0; n < D / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            ds[n][e] = dfinal ? __ldg(dfinal + state_at + int64_t(8 * n + 2 * (lane & 3) + (e & 1)) * dv + (e >> 1) * 8) : 0.f;
+            // the gradient behind the sequence; a segment that is not the last starts from zero in the first launch
+            ds[n][e] = dfinal && (!LOCAL || behind == 0) ? __ldg(dfinal + state_at + int64_t(8 * n + 2 * (lane & 3) + (e & 1)) * dv + (e >> 1) * 8) : 0.f;
+    // the gradient behind an earlier segment: dS <- M^T dS + B over the segments behind it.  The last one's B already has dfinal.
+    if (!LOCAL)
+        for (int later = behind; later > 0; --later) {
+            const int64_t place = (int64_t(blockIdx.x) + later) * shape.heads + head;
+            const float4* end = reinterpret_cast<const float4*>(ends + place * D * dv) + column / 16 * (D / 8) * 32 + lane;
+            float x[D / 8][4];
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float4*>(x[n]) = __ldg(end + n * 32);
+            if (later < behind) {
+                load_block<2 * D * D, THREADS>(base, reinterpret_cast<const char*>(shape.segments.m + place * D * D), thread);
+                cp_async_commit();
+                cp_async_wait<0>();
+                __syncthreads();
+#pragma unroll
+                for (int kb = 0; kb < D / 16; ++kb) {
+                    unsigned a[4];
+                    to_operand(a, ds[2 * kb], ds[2 * kb + 1]);
+#pragma unroll
+                    for (int np = 0; np < D / 16; ++np) {
+                        unsigned b[4];
+                        ldsm4(b, base + (np * 2 * (D / 8) + kb * 2) * 128 + cols_first_blocked(lane, D / 8));
+                        mma16816(x[2 * np], a, b[0], b[1]);
+                        mma16816(x[2 * np + 1], a, b[2], b[3]);
+                    }
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ds[n][e] = x[n][e];
+        }
     if (chunks > 0) load(chunks - 1);
     for (int c = chunks - 1; c >= 0; --c) {
         cp_async_wait<0>();
         __syncthreads();  // chunk c is in, and every warp has left chunk c + 1
-        {  // X of this chunk, transposed: the warp's own rows, two kilobytes, needed only after dU
+        if (!LOCAL) {  // X of this chunk, transposed: the warp's own rows, two kilobytes, needed only after dU
             const char* from = reinterpret_cast<const char*>(saved.x + ((slot + c) * shape.heads + head) * CHUNK * dv + column * CHUNK);
 #pragma unroll
             for (int i = lane * 16; i < 2048; i += 512)
@@ -94,8 +143,10 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
         for (int kb = 0; kb < D / 16; ++kb) {
             unsigned a[4];
             to_operand(a, ds[2 * kb], ds[2 * kb + 1]);
-            unsigned* to = state_out + 2 * kb * 32;
-            to[0] = a[0], to[D / 8 * 32] = a[1], to[32] = a[2], to[D / 8 * 32 + 32] = a[3];
+            if (!LOCAL) {
+                unsigned* to = state_out + 2 * kb * 32;
+                to[0] = a[0], to[D / 8 * 32] = a[1], to[32] = a[2], to[D / 8 * 32 + 32] = a[3];
+            }
 #pragma unroll
             for (int np = 0; np < TILES / 2; ++np) {
                 unsigned b[4];
@@ -133,17 +184,19 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
         __syncwarp();
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np) {
-            unsigned xx[4];
+            unsigned xx[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) xx[e] = *reinterpret_cast<const unsigned*>(shared + Stage::X + warp * 2048 + ((e & 1) * TILES + 2 * np + (e >> 1)) * 128 + lane * 4);
+            for (int e = 0; e < 4 && !LOCAL; ++e) xx[e] = *reinterpret_cast<const unsigned*>(shared + Stage::X + warp * 2048 + ((e & 1) * TILES + 2 * np + (e >> 1)) * 128 + lane * 4);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float(&tile)[4] = du[2 * np + h];
-                float even = tile[0] * low_half(xx[2 * h]) + tile[2] * low_half(xx[2 * h + 1]);
-                float odd = tile[1] * high_half(xx[2 * h]) + tile[3] * high_half(xx[2 * h + 1]);
+                if (!LOCAL) {
+                    float even = tile[0] * low_half(xx[2 * h]) + tile[2] * low_half(xx[2 * h + 1]);
+                    float odd = tile[1] * high_half(xx[2 * h]) + tile[3] * high_half(xx[2 * h + 1]);
 #pragma unroll
-                for (int m = 4; m < 32; m <<= 1) even += __shfl_xor_sync(FULL, even, m), odd += __shfl_xor_sync(FULL, odd, m);
-                if (lane < 4) *reinterpret_cast<float2*>(part + 16 * np + 8 * h + 2 * lane) = make_float2(even, odd);
+                    for (int m = 4; m < 32; m <<= 1) even += __shfl_xor_sync(FULL, even, m), odd += __shfl_xor_sync(FULL, odd, m);
+                    if (lane < 4) *reinterpret_cast<float2*>(part + 16 * np + 8 * h + 2 * lane) = make_float2(even, odd);
+                }
                 const float2 b = *reinterpret_cast<const float2*>(rows + CHUNK + 16 * np + 8 * h + 2 * (lane & 3));
                 tile[0] *= b.x, tile[1] *= b.y, tile[2] *= b.x, tile[3] *= b.y;
             }
@@ -163,23 +216,25 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
                 mma16816(dy[2 * np], dx[kb], b[0], b[1]);
                 mma16816(dy[2 * np + 1], dx[kb], b[2], b[3]);
             }
-        // dV leaves through the warp's room of X: rows of 32 bytes, the halves of rows 4-7 of every eight exchanged
-        const unsigned values = base + Stage::X + warp * 2048 + ((lane & 7) + ((lane >> 4) << 3)) * 32 + ((((lane >> 3) ^ (lane >> 2)) & 1) * 16);
-        __syncwarp();
+        if (!LOCAL) {
+            // dV leaves through the warp's room of X: rows of 32 bytes, the halves of rows 4-7 of every eight exchanged
+            const unsigned values = base + Stage::X + warp * 2048 + ((lane & 7) + ((lane >> 4) << 3)) * 32 + ((((lane >> 3) ^ (lane >> 2)) & 1) * 16);
+            __syncwarp();
 #pragma unroll
-        for (int np = 0; np < TILES / 2; ++np)
-            stsm4_trans(values + np * 512, pack2(dy[2 * np][0], dy[2 * np][1]), pack2(dy[2 * np][2], dy[2 * np][3]),
-                        pack2(dy[2 * np + 1][0], dy[2 * np + 1][1]), pack2(dy[2 * np + 1][2], dy[2 * np + 1][3]));
-        __syncwarp();
-        const int count = min(CHUNK, length - c * CHUNK);
-        char* to = reinterpret_cast<char*>(dv_out + ((row + int64_t(c) * CHUNK) * shape.heads + head) * dv + column);
+            for (int np = 0; np < TILES / 2; ++np)
+                stsm4_trans(values + np * 512, pack2(dy[2 * np][0], dy[2 * np][1]), pack2(dy[2 * np][2], dy[2 * np][3]),
+                            pack2(dy[2 * np + 1][0], dy[2 * np + 1][1]), pack2(dy[2 * np + 1][2], dy[2 * np + 1][3]));
+            __syncwarp();
+            const int count = min(CHUNK, length - c * CHUNK);
+            char* to = reinterpret_cast<char*>(dv_out + ((row + int64_t(c) * CHUNK) * shape.heads + head) * dv + column);
 #pragma unroll
-        for (int i = 0; i < CHUNK * 2 / 32; ++i) {
-            const int t = i * 16 + (lane >> 1);
-            const uint4 piece = *reinterpret_cast<const uint4*>(shared + Stage::X + warp * 2048 + t * 32 + (((lane & 1) ^ ((t >> 2) & 1)) * 16));
-            if (t < count) *reinterpret_cast<uint4*>(to + t * value_stride + (lane & 1) * 16) = piece;
+            for (int i = 0; i < CHUNK * 2 / 32; ++i) {
+                const int t = i * 16 + (lane >> 1);
+                const uint4 piece = *reinterpret_cast<const uint4*>(shared + Stage::X + warp * 2048 + t * 32 + (((lane & 1) ^ ((t >> 2) & 1)) * 16));
+                if (t < count) *reinterpret_cast<uint4*>(to + t * value_stride + (lane & 1) * 16) = piece;
+            }
+            __syncwarp();  // the room is free for the next chunk's X
         }
-        __syncwarp();  // the room is free for the next chunk's X
         // scale e^G dO and -e^G dY, the left operands of the state's step
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np) {
@@ -214,7 +269,11 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
                 mma16816(ds[2 * np + 1], grad[kb], b[2], b[3]);
             }
     }
-    if (dinitial) {
+    if (LOCAL) {
+        float4* to = reinterpret_cast<float4*>(ends + (int64_t(blockIdx.x) * shape.heads + head) * D * dv) + column / 16 * (D / 8) * 32 + lane;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) to[n * 32] = *reinterpret_cast<float4*>(ds[n]);
+    } else if (dinitial && number == 0) {
 #pragma unroll
         for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -251,6 +310,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_kernel(Del
     int64_t row;
     int count;
     const int64_t slot = blockIdx.x;
+    if (shape.layout.cu && key_head == 0) clear_gradients<GRADIENT_THREADS>(shape, dq, dk, dg, dbeta, blockIdx.x, gridDim.x, thread);
     shape.layout.chunk(slot, row, count);
     if (count == 0) return;
     const unsigned base = smem_address(shared);
@@ -537,22 +597,25 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_kernel(Del
     }
 }
 
-template <int D, int WARPS>
+template <int D, int WARPS, bool LOCAL = false>
 cudaError_t launch_reverse(const DeltaShape& shape, const DeltaGradients& x, const DeltaSaved& saved, cudaStream_t stream) {
+    if constexpr (!LOCAL && D >= 64 && WARPS == 4)
+        if (shape.segments.length)
+            if (cudaError_t status = launch_reverse<D, WARPS, true>(shape, x, saved, stream)) return status;
     constexpr int BYTES = ReverseStage<D, WARPS>::TOTAL;
-    auto* kernel = delta_reverse_kernel<D, WARPS>;
-    if (cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES)) return status;
-    KernelTimer timer("delta_reverse", stream);
-    kernel<<<dim3(shape.layout.sequences, shape.heads, shape.dv / (16 * WARPS)), WARPS * 32, BYTES, stream>>>(
-        shape, x.q, x.k, x.dout, x.dfinal, saved, x.dstates, x.dbeta_parts, x.dv, x.dinitial);
+    constexpr auto* kernel = delta_reverse_kernel<D, WARPS, LOCAL>;
+    if (cudaError_t status = allow_shared<kernel>(BYTES)) return status;
+    KernelTimer timer(LOCAL ? "delta_reverse_segments" : "delta_reverse", stream);
+    kernel<<<dim3(unsigned(shape.segments.count(shape.layout)), shape.heads, shape.dv / (16 * WARPS)), WARPS * 32, BYTES, stream>>>(
+        shape, x.q, x.k, x.dout, x.dfinal, saved, x.dstates, x.dbeta_parts, x.dv, x.dinitial, x.ends);
     return cudaGetLastError();
 }
 
 template <int D, int DV>
 cudaError_t launch_gradient(const DeltaShape& shape, const DeltaGradients& x, const DeltaSaved& saved, cudaStream_t stream) {
     constexpr int BYTES = GradientShared<D, DV>::BYTES;
-    auto* kernel = delta_gradient_kernel<D, DV>;
-    if (cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES)) return status;
+    constexpr auto* kernel = delta_gradient_kernel<D, DV>;
+    if (cudaError_t status = allow_shared<kernel>(BYTES)) return status;
     KernelTimer timer("delta_gradient", stream);
     kernel<<<dim3(unsigned(shape.layout.slots()), shape.key_heads), GRADIENT_THREADS, BYTES, stream>>>(
         shape, x.q, x.k, x.dout, x.dv, saved, x.dstates, x.dbeta_parts, x.dq, x.dk, x.dg, x.dbeta);

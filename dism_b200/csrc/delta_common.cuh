@@ -15,9 +15,24 @@
 // the next product.  Everything that depends on the state is computed transposed ([dv, position] and [dv, d]), so a warp
 // owns 16 columns of the state for the whole sequence and the chain of products never leaves its registers.
 #pragma once
+#include <atomic>
+
 #include "dism_common.cuh"
 
 namespace dism {
+
+// Opts a kernel into its dynamic shared memory, once per device (the call costs a microsecond of host time).
+template <auto* KERNEL>
+cudaError_t allow_shared(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int device = 0;
+    if (cudaError_t status = cudaGetDevice(&device)) return status;
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    if (cudaError_t status = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return status;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return cudaSuccess;
+}
 
 constexpr int CHUNK = 64;
 // Per chunk and head: e^G, b, e^{G_63 - G}, the product of the last two, and G as a pair of floats.
@@ -76,6 +91,13 @@ __device__ __forceinline__ unsigned rows_first_tile(int lane) { return rows_firs
 __device__ __forceinline__ unsigned cols_first_tile(int lane) { return lane * 16; }
 __host__ __device__ constexpr int tile_at(int row_tile, int column_tile) { return (row_tile * (row_tile + 1) / 2 + column_tile) * 512; }
 
+// Zeros in the rows of no document, before the first and behind the last: `pieces` of 16 bytes from `tensor` on in each row.
+template <int THREADS>
+__device__ __forceinline__ void clear_rows(char* tensor, int64_t stride, int pieces, int64_t first, int64_t last, int thread) {
+    for (int64_t i = thread; i < (last - first) * pieces; i += THREADS)
+        *reinterpret_cast<uint4*>(tensor + (first + i / pieces) * stride + i % pieces * 16) = make_uint4(0, 0, 0, 0);
+}
+
 // Where the sequences lie.  Fixed layout: `sequences` rows of n positions.  Packed: one row of n positions, document i at
 // [cu[i], cu[i+1]).  Every chunk has a slot of its own: in a pack, document i starts at slot cu[i] / 64 + i, which leaves
 // room for its last, partly filled chunk and needs no running sum over the documents.  Entries of cu are clamped to the
@@ -116,12 +138,67 @@ struct DeltaLayout {
     }
 };
 
+// A chain of chunks is cut into segments of `length` chunks (0: not cut) when there are too few chains to fill the device.  The state is
+// linear in the state at the segment's start, S_end = M S_start + B, so a first launch finds M (the chain applied to the unit matrix
+// without values) and B (the chain from zero) of all segments but the last of a sequence at once, and a second one runs every segment
+// from its true start, which it puts together from the M and B before it.  Segments are numbered like chunks: in a pack, document i
+// begins at segment slot / length + i.
+struct DeltaSegments {
+    int length;
+    float* ends;                  // B as accumulator fragments, [segments, H, D * DV]
+    __nv_bfloat16 *m, *m_rest;    // M, transposed, in 8 x 8 blocks, [segments, H, D * D]; the remainders only for an exact state
+    __host__ __device__ int64_t count(const DeltaLayout& layout) const {
+        if (!length) return layout.sequences;
+        if (!layout.cu) return int64_t(layout.sequences) * ((layout.chunks() + length - 1) / length);
+        return layout.slots() / length + layout.sequences;
+    }
+    // Sequence and number in it of a segment.
+    __device__ void find(const DeltaLayout& layout, int64_t segment, int& sequence, int& number) const {
+        number = 0;
+        if (!length) {
+            sequence = int(segment);
+        } else if (!layout.cu) {
+            const int each = (layout.chunks() + length - 1) / length;
+            sequence = int(segment / each), number = int(segment % each);
+        } else {
+            int lo = 0, hi = layout.sequences - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if ((layout.start(mid) / CHUNK + mid) / length + mid <= segment) lo = mid;
+                else hi = mid - 1;
+            }
+            sequence = lo, number = int(segment - ((layout.start(lo) / CHUNK + lo) / length + lo));
+        }
+    }
+};
+
 struct DeltaShape {
     DeltaLayout layout;
+    DeltaSegments segments;
     int key_heads, heads, d, dv;
     bool gates_bf16;
     float scale;
 };
+
+// Zeros in the gradients' rows of no document; CTA `index` of `count` takes every count-th row.
+template <int THREADS>
+__device__ __forceinline__ void clear_gradients(const DeltaShape& shape, __nv_bfloat16* dq, __nv_bfloat16* dk, void* dg, void* dbeta, int64_t index,
+                                                int64_t count, int thread) {
+    const int64_t begin = shape.layout.start(0), end = shape.layout.start(shape.layout.sequences), outside = begin + max(int64_t(shape.layout.n) - end, int64_t(0));
+    const int width = shape.key_heads * shape.d;
+    for (int64_t i = index; i < outside; i += count) {
+        const int64_t row = i < begin ? i : end + i - begin;
+        for (int j = thread * 8; j < width; j += THREADS * 8) {
+            *reinterpret_cast<uint4*>(dq + row * width + j) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(dk + row * width + j) = make_uint4(0, 0, 0, 0);
+        }
+        for (int j = thread; j < shape.heads; j += THREADS) {
+            const int64_t at = row * shape.heads + j;
+            if (shape.gates_bf16) static_cast<__nv_bfloat16*>(dg)[at] = static_cast<__nv_bfloat16*>(dbeta)[at] = __float2bfloat16(0.f);
+            else static_cast<float*>(dg)[at] = static_cast<float*>(dbeta)[at] = 0.f;
+        }
+    }
+}
 
 // What the kernels hand to one another, per slot and value head.  The backward needs all of it.
 struct DeltaSaved {
@@ -200,11 +277,14 @@ __device__ __forceinline__ void load_block(unsigned tile, const char* global, in
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tile + i), "l"(global + i));
 }
 
+// Chunks to a segment, 0 for whole sequences.
+int delta_segment_length(const DeltaLayout& layout, int heads, int d, int dv);
 struct DeltaGradients {
     const __nv_bfloat16 *q, *k, *dout;
     const float* dfinal;  // gradient of the last states, or null
     __nv_bfloat16* dstates;  // scratch: dS1 [slots, H, DV, D] blocked
     float* dbeta_parts;      // scratch: [DV / 16, slots, H, CHUNK]
+    float* ends;             // scratch: the reverse chain's B, as DeltaSegments has the forward's
     __nv_bfloat16 *dq, *dk, *dv;
     void *dg, *dbeta;        // in the gates' type
     float* dinitial;         // gradient of the first states, or null

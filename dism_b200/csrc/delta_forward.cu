@@ -8,6 +8,7 @@
 // EXACT: the state is wanted at the end.  S0 in S0 K^T, Y, T and U are then kept as bf16 pairs (value and remainder, 16 bits),
 // which holds the state to a few 1e-6; without it a single bf16 is enough for outputs that are bf16 themselves.
 #include "delta_common.cuh"
+#include <cstdlib>
 
 namespace dism {
 namespace {
@@ -20,7 +21,8 @@ struct ForwardStage {
     static constexpr int BYTES = ROWS + 3 * CHUNK * 4;
 };
 
-template <int D, int WARPS, bool EXACT, bool SAVE>
+// LOCAL: the first launch over segments (see DeltaSegments): neither Q nor outputs, B from the first CTAs of a head and M from the others.
+template <int D, int WARPS, bool EXACT, bool SAVE, bool LOCAL>
 __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape shape, const __nv_bfloat16* __restrict__ q,
                                                                  const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v,
                                                                  const float* __restrict__ initial, DeltaSaved saved,
@@ -29,13 +31,30 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
     constexpr int THREADS = WARPS * 32, TILES = CHUNK / 8;
     extern __shared__ __align__(128) unsigned char shared[];
     const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
-    const int head = blockIdx.y, sequence = blockIdx.x, dv = shape.dv;
-    const int key_head = head / (shape.heads / shape.key_heads), column = (blockIdx.z * WARPS + warp) * 16;
+    const int head = blockIdx.y, dv = shape.dv, key_head = head / (shape.heads / shape.key_heads);
+    const bool unit = LOCAL && blockIdx.z * WARPS * 16 >= dv;  // this CTA's columns are the unit matrix's
+    const int column = (blockIdx.z * WARPS + warp) * 16 - (unit ? dv : 0);
     int64_t row, slot;
-    int length;
+    int length, sequence, number;
+    shape.segments.find(shape.layout, blockIdx.x, sequence, number);
     shape.layout.span(sequence, row, length, slot);
-    const int chunks = (length + CHUNK - 1) / CHUNK;
     const unsigned base = smem_address(shared);
+    if (!LOCAL && shape.layout.cu && number == 0) {
+        char* to = reinterpret_cast<char*>(out + int64_t(head) * dv + blockIdx.z * WARPS * 16);
+        const int64_t stride = int64_t(shape.heads) * dv * 2;
+        if (sequence == 0) clear_rows<WARPS * 32>(to, stride, WARPS * 2, 0, row, thread);
+        if (sequence == shape.layout.sequences - 1) clear_rows<WARPS * 32>(to, stride, WARPS * 2, row + length, shape.layout.n, thread);
+    }
+    int chunks = (length + CHUNK - 1) / CHUNK;
+    bool last = true;
+    if (shape.segments.length) {
+        const int before = min(number * shape.segments.length, chunks);
+        last = chunks - before <= shape.segments.length;
+        if (number && before == chunks) return;  // no such segment
+        if (LOCAL && last) return;
+        chunks = min(chunks - before, shape.segments.length);
+        slot += before, row += int64_t(before) * CHUNK, length -= before * CHUNK;
+    }
 
     const int64_t key_stride = int64_t(shape.key_heads) * D * 2, value_stride = int64_t(shape.heads) * dv * 2;
     auto load = [&](int c) {
@@ -44,14 +63,14 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
         const int64_t at = row + int64_t(c) * CHUNK, place = (slot + c) * shape.heads + head;
         const int64_t key = (at * shape.key_heads + key_head) * D * 2;
         load_tile<2 * D, THREADS>(stage + Stage::K, reinterpret_cast<const char*>(k) + key, key_stride, count, thread);
-        load_tile<32 * WARPS, THREADS>(stage + Stage::V,
+        if (!unit) load_tile<32 * WARPS, THREADS>(stage + Stage::V,
                                        reinterpret_cast<const char*>(v) + ((at * shape.heads + head) * dv + blockIdx.z * WARPS * 16) * 2,
                                        value_stride, count, thread);
         load_block<3 * CHUNK * 4, THREADS>(stage + Stage::ROWS, reinterpret_cast<const char*>(saved.rows + place * ROW_VALUES), thread);
         load_block<2 * MATRIX, THREADS>(stage + Stage::T, reinterpret_cast<const char*>(saved.t + place * MATRIX), thread);
         if (EXACT) load_block<2 * MATRIX, THREADS>(stage + Stage::T_REST, reinterpret_cast<const char*>(saved.t_rest + place * MATRIX), thread);
-        load_tile<2 * D, THREADS>(stage + Stage::Q, reinterpret_cast<const char*>(q) + key, key_stride, count, thread);
-        load_block<2 * MATRIX, THREADS>(stage + Stage::P, reinterpret_cast<const char*>(saved.p + place * MATRIX), thread);
+        if (!LOCAL) load_tile<2 * D, THREADS>(stage + Stage::Q, reinterpret_cast<const char*>(q) + key, key_stride, count, thread);
+        if (!LOCAL) load_block<2 * MATRIX, THREADS>(stage + Stage::P, reinterpret_cast<const char*>(saved.p + place * MATRIX), thread);
         cp_async_commit();
     };
 
@@ -60,8 +79,51 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
 #pragma unroll
     for (int n = 0; n < D / 8; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            s[n][e] = initial ? __ldg(initial + state_at + int64_t(8 * n + 2 * (lane & 3) + (e & 1)) * dv + (e >> 1) * 8) : 0.f;
+        for (int e = 0; e < 4; ++e) {
+            const int d = 8 * n + 2 * (lane & 3) + (e & 1);
+            if (LOCAL) s[n][e] = unit && d == column + (lane >> 2) + (e >> 1) * 8 ? 1.f : 0.f;
+            else s[n][e] = initial ? __ldg(initial + state_at + int64_t(d) * dv + (e >> 1) * 8) : 0.f;
+        }
+    // the state at a later segment's start: S <- M S + B over the segments before it
+    if (!LOCAL)
+        for (int before = 0; before < number; ++before) {
+            const int64_t place = (int64_t(blockIdx.x) - number + before) * shape.heads + head;
+            load_block<2 * D * D, THREADS>(base, reinterpret_cast<const char*>(shape.segments.m + place * D * D), thread);
+            if (EXACT) load_block<2 * D * D, THREADS>(base + 2 * D * D, reinterpret_cast<const char*>(shape.segments.m_rest + place * D * D), thread);
+            cp_async_commit();
+            float x[D / 8][4];
+            const float4* end = reinterpret_cast<const float4*>(shape.segments.ends + place * D * dv) + column / 16 * (D / 8) * 32 + lane;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float4*>(x[n]) = __ldg(end + n * 32);
+            cp_async_wait<0>();
+            __syncthreads();
+#pragma unroll
+            for (int kb = 0; kb < D / 16; ++kb) {
+                unsigned a[4], rest[4];
+                to_operand(a, s[2 * kb], s[2 * kb + 1]);
+                if (EXACT) to_operand_rest(rest, a, s[2 * kb], s[2 * kb + 1]);
+                const unsigned m = base + kb * 2 * (D / 8) * 128 + rows_first_blocked(lane, D / 8);
+#pragma unroll
+                for (int np = 0; np < D / 16; ++np) {
+                    unsigned b[4];
+                    ldsm4_trans(b, m + np * 256);
+                    mma16816(x[2 * np], a, b[0], b[1]);
+                    mma16816(x[2 * np + 1], a, b[2], b[3]);
+                    if (EXACT) {
+                        mma16816(x[2 * np], rest, b[0], b[1]);
+                        mma16816(x[2 * np + 1], rest, b[2], b[3]);
+                        ldsm4_trans(b, m + 2 * D * D + np * 256);
+                        mma16816(x[2 * np], a, b[0], b[1]);
+                        mma16816(x[2 * np + 1], a, b[2], b[3]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] = x[n][e];
+            __syncthreads();
+        }
     if (chunks > 0) load(0);
     for (int c = 0; c < chunks; ++c) {
         cp_async_wait<0>();
@@ -96,9 +158,11 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
                     mma16816(ks[2 * np], rest, b[0], b[1]);
                     mma16816(ks[2 * np + 1], rest, b[2], b[3]);
                 }
-                ldsm4(b, keys.at(kb * 32) + Stage::Q - Stage::K + np * 16 * Stage::PITCH);
-                mma16816(qs[2 * np], a, b[0], b[1]);
-                mma16816(qs[2 * np + 1], a, b[2], b[3]);
+                if (!LOCAL) {
+                    ldsm4(b, keys.at(kb * 32) + Stage::Q - Stage::K + np * 16 * Stage::PITCH);
+                    mma16816(qs[2 * np], a, b[0], b[1]);
+                    mma16816(qs[2 * np + 1], a, b[2], b[3]);
+                }
             }
         }
         // Y, as the left operand of X = T Y
@@ -106,8 +170,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
         unsigned y[TILES / 2][4], y_rest[EXACT ? TILES / 2 : 1][4];
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np) {
-            unsigned vv[4];
-            ldsm4_trans(vv, values + np * 16 * Stage::VALUE_PITCH);
+            unsigned vv[4] = {0, 0, 0, 0};
+            if (!unit) ldsm4_trans(vv, values + np * 16 * Stage::VALUE_PITCH);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float(&tile)[4] = ks[2 * np + h];
@@ -175,8 +239,9 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
                 float(&tile)[4] = x[2 * np + h];
                 tile[0] *= b.x, tile[1] *= b.y, tile[2] *= b.x, tile[3] *= b.y;
             }
-            to_operand(u[np], x[2 * np], x[2 * np + 1]);
+            if (!LOCAL) to_operand(u[np], x[2 * np], x[2 * np + 1]);
         }
+        if (!LOCAL) {
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np)
 #pragma unroll
@@ -187,6 +252,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
                 mma16816(qs[2 * np + 1], u[kb], b[2], b[3]);
             }
         leave(qs, reinterpret_cast<char*>(out + ((row + int64_t(c) * CHUNK) * shape.heads + head) * dv + column), value_stride, count);
+        }
         const float kept = rows[CHUNK - 1];
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np) {
@@ -218,7 +284,25 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
                 }
             }
     }
-    if (final_state) {
+    if (LOCAL) {
+        const int64_t place = int64_t(blockIdx.x) * shape.heads + head;
+        if (unit) {
+            unsigned* to = reinterpret_cast<unsigned*>(shape.segments.m + place * D * D) + int64_t(column / 8) * (D / 8) * 32 + lane;
+            unsigned* to_rest = reinterpret_cast<unsigned*>(shape.segments.m_rest + place * D * D) + int64_t(column / 8) * (D / 8) * 32 + lane;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const unsigned value = pack2(s[n][2 * h], s[n][2 * h + 1]);
+                    to[(h * (D / 8) + n) * 32] = value;
+                    if (EXACT) to_rest[(h * (D / 8) + n) * 32] = pack2_rest(s[n][2 * h], s[n][2 * h + 1], value);
+                }
+        } else {
+            float4* to = reinterpret_cast<float4*>(shape.segments.ends + place * D * dv) + column / 16 * (D / 8) * 32 + lane;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) to[n * 32] = *reinterpret_cast<float4*>(s[n]);
+        }
+    } else if (final_state && last) {
 #pragma unroll
         for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -227,14 +311,15 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
     }
 }
 
-template <int D, int WARPS, bool EXACT, bool SAVE>
+template <int D, int WARPS, bool EXACT, bool SAVE, bool LOCAL = false>
 cudaError_t launch(const DeltaShape& shape, const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v,
                    const float* initial, const DeltaSaved& saved, __nv_bfloat16* out, float* final_state, cudaStream_t stream) {
     constexpr int BYTES = 2 * ForwardStage<D, WARPS, EXACT>::BYTES;
-    auto* kernel = delta_chain_kernel<D, WARPS, EXACT, SAVE>;
-    if (cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES)) return status;
-    KernelTimer timer("delta_chain", stream);
-    kernel<<<dim3(shape.layout.sequences, shape.heads, shape.dv / (16 * WARPS)), WARPS * 32, BYTES, stream>>>(shape, q, k, v, initial, saved, out, final_state);
+    constexpr auto* kernel = delta_chain_kernel<D, WARPS, EXACT, SAVE, LOCAL>;
+    if (cudaError_t status = allow_shared<kernel>(BYTES)) return status;
+    KernelTimer timer(LOCAL ? "delta_segments" : "delta_chain", stream);
+    const dim3 grid(unsigned(shape.segments.count(shape.layout)), shape.heads, (shape.dv + (LOCAL ? D : 0)) / (16 * WARPS));
+    kernel<<<grid, WARPS * 32, BYTES, stream>>>(shape, q, k, v, initial, saved, out, final_state);
     return cudaGetLastError();
 }
 
@@ -242,6 +327,13 @@ template <int D, int WARPS>
 cudaError_t choose(const DeltaShape& shape, const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v,
                    const float* initial, const DeltaSaved& saved, __nv_bfloat16* out, float* final_state, cudaStream_t stream) {
     const bool exact = saved.t_rest != nullptr, save = saved.states != nullptr;
+    if constexpr (D >= 64 && WARPS == 4) {
+        if (shape.segments.length) {
+            cudaError_t status = exact ? launch<D, WARPS, true, false, true>(shape, q, k, v, initial, saved, out, final_state, stream)
+                                       : launch<D, WARPS, false, false, true>(shape, q, k, v, initial, saved, out, final_state, stream);
+            if (status) return status;
+        }
+    }
     if (exact && save) return launch<D, WARPS, true, true>(shape, q, k, v, initial, saved, out, final_state, stream);
     if (exact) return launch<D, WARPS, true, false>(shape, q, k, v, initial, saved, out, final_state, stream);
     if (save) return launch<D, WARPS, false, true>(shape, q, k, v, initial, saved, out, final_state, stream);
@@ -255,6 +347,16 @@ cudaError_t by_width(const DeltaShape& shape, const __nv_bfloat16* q, const __nv
     return choose<D, 2>(shape, q, k, v, initial, saved, out, final_state, stream);
 }
 }  // namespace
+
+int delta_segment_length(const DeltaLayout& layout, int heads, int d, int dv) {
+    if (d < 64 || dv < 64) return 0;
+    static const int least = getenv("DELTA_LEAST") ? atoi(getenv("DELTA_LEAST")) : 8, ratio = getenv("DELTA_RATIO") ? atoi(getenv("DELTA_RATIO")) : 3;
+    static const double scale = getenv("DELTA_SCALE") ? atof(getenv("DELTA_SCALE")) : 1.;
+    const int sms = device_sm_count();
+    const int64_t chains = int64_t(heads) * (dv / 64), even = sms > 0 ? int64_t(scale * double(layout.slots() * chains + sms - 1) / sms) : 1 << 30;
+    const int64_t length = even < least ? least : even;
+    return ratio * length <= layout.chunks() ? int(length) : 0;
+}
 
 cudaError_t launch_delta_chain(const DeltaShape& shape, const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v,
                                const float* initial, const DeltaSaved& saved, __nv_bfloat16* out, float* final_state,

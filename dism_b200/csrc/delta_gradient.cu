@@ -87,6 +87,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
     const int64_t units = shape.layout.slots() * shape.key_heads;
     int64_t row = 0, next_row = 0, unit = blockIdx.x, next_unit;
     int count = 0, next_count = 0;
+    if (shape.layout.cu) clear_gradients<GRADIENT_THREADS>(shape, dq, dk, dg, dbeta, blockIdx.x, gridDim.x, thread);
     // the first unit from `from` on that has positions
     auto find = [&](int64_t from, int64_t& at, int& positions) {
         for (; from < units; from += gridDim.x) {
@@ -367,8 +368,8 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
 template <int D, int DV>
 cudaError_t launch(const DeltaShape& shape, const DeltaGradients& x, const DeltaSaved& saved, cudaStream_t stream) {
     constexpr int BYTES = GradientTiles<D, DV>::BYTES;
-    auto* kernel = delta_gradient_tensor_kernel<D, DV>;
-    if (cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES)) return status;
+    constexpr auto* kernel = delta_gradient_tensor_kernel<D, DV>;
+    if (cudaError_t status = allow_shared<kernel>(BYTES)) return status;
     KernelTimer timer("delta_gradient", stream);
     const int64_t units = shape.layout.slots() * shape.key_heads;
     kernel<<<unsigned(units < device_sm_count() ? units : device_sm_count()), GRADIENT_THREADS, BYTES, stream>>>(

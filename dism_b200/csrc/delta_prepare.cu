@@ -253,7 +253,7 @@ template <int D>
 cudaError_t launch(const DeltaShape& shape, const __nv_bfloat16* q, const __nv_bfloat16* k, const void* g, const void* beta,
                    const DeltaSaved& saved, cudaStream_t stream) {
     constexpr int BYTES = PrepareShared<D>::BYTES;
-    if (cudaError_t status = cudaFuncSetAttribute(delta_prepare_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES)) return status;
+    if (cudaError_t status = allow_shared<delta_prepare_kernel<D>>(BYTES)) return status;
     KernelTimer timer("delta_prepare", stream);
     delta_prepare_kernel<D><<<dim3(unsigned(shape.layout.slots()), shape.heads), PREPARE_THREADS, BYTES, stream>>>(shape, q, k, g, beta, saved);
     return cudaGetLastError();

@@ -18,6 +18,7 @@ Beyond the reference's module: labels, labels_pair, longest_match, the gated del
 delta_step) and dropout.
 """
 import contextlib
+import functools
 
 import torch
 
@@ -475,22 +476,40 @@ def longest_match(streams):
 # ---- gated delta rule ------------------------------------------------------------------------------
 # The reference's hybrid layers (dism_v3/python/flash_dism/hybrid_gdn.py, pure_gdn.py) take this mixer from an outside
 # package; here it is part of the library, in the layouts of the other operators.
+_nothing = contextlib.nullcontext()
+
+
+def _on(device):
+    """Makes `device` current for the calls inside; free when it is already."""
+    return _nothing if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _raw_stream(tensor):
+    return _current_stream(tensor.device.index)
+
+
+_current_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_delta_saved_bytes = functools.lru_cache(256)(_abi.dism_delta_saved)
+_delta_workspace_bytes = functools.lru_cache(256)(_abi.dism_delta_backward_workspace)
+
+
 def _delta_operands(q, k, v, g, beta, tail):
     """Checks q, k [*,HK,D], v [*,H,DV], g and beta [*,H]; returns (HK, H, D, DV, gates are bf16)."""
     _check(v, torch.bfloat16, None, 'v')
     if v.dim() != tail + 2:
         _fail('v must be [B,N,H,DV]' if tail == 2 else 'v must be [B,H,DV]')
     _check(q, torch.bfloat16, None, 'q')
-    if q.dim() != v.dim() or q.shape[:tail] != v.shape[:tail] or q.device != v.device:
+    rows, keys = v.shape[:-1], q.shape
+    if len(keys) != tail + 2 or keys[:-2] != rows[:-1]:
         _fail('q: invalid device, dtype, shape or stride')
-    _check(k, torch.bfloat16, q.shape, 'k')
+    _check(k, torch.bfloat16, keys, 'k')
     if not torch.is_tensor(g) or g.dtype not in (torch.float32, torch.bfloat16):
         _fail('g must be float32 or bfloat16')
-    _check(g, g.dtype, v.shape[:-1], 'g')
-    _check(beta, g.dtype, v.shape[:-1], 'beta')
-    if any(x.device != v.device for x in (k, g, beta)):
+    _check(g, g.dtype, rows, 'g')
+    _check(beta, g.dtype, rows, 'beta')
+    if not q.device == k.device == g.device == beta.device == v.device:
         _fail('operands on different devices')
-    key_heads, d, heads, dv = q.size(-2), q.size(-1), v.size(-2), v.size(-1)
+    key_heads, d, heads, dv = keys[-2], keys[-1], rows[-1], v.size(-1)
     if heads <= 0 or key_heads <= 0 or heads % key_heads:
         _fail('value heads must be a multiple of the key heads')
     if d not in (32, 64, 128) or dv not in (32, 64, 128):
@@ -519,10 +538,9 @@ def _delta_state(state, sequences, heads, d, dv, device, name):
     return state.data_ptr()
 
 
-def delta_forward(x, scale, initial_state=None, final_state=False, cu_seqlens=None, covered=True, backward=False):
+def delta_forward(x, scale, initial_state=None, final_state=False, cu_seqlens=None, backward=False):
     """x = (q, k bf16 [B,N,HK,D], v bf16 [B,N,H,DV], g, beta float or bf16 [B,N,H]) -> (out bf16 [B,N,H,DV], final state FP32
-    [sequences,H,D,DV] or None, saved buffer).  `covered`: the sequences are known to cover every row; otherwise rows of none are zeros.
-    With backward=True the saved buffer is what delta_backward needs; otherwise it is dead."""
+    [sequences,H,D,DV] or None, saved buffer).  Rows before the first and behind the last sequence of a pack are zeros.  With backward=True the saved buffer is what delta_backward needs; otherwise it is dead."""
     if len(x) != 5:
         _fail('expected q,k,v,g,beta')
     q, k, v, g, beta = x
@@ -530,23 +548,23 @@ def delta_forward(x, scale, initial_state=None, final_state=False, cu_seqlens=No
     sequences, starts = _delta_sequences(v, cu_seqlens)
     initial = _delta_state(initial_state, sequences, heads, d, dv, v.device, 'initial state')
     n = v.size(1)
-    with torch.cuda.device(v.device):
-        out = (torch.empty_like if covered else torch.zeros_like)(v)
+    with _on(v.device):
+        out = torch.empty_like(v)
         final = torch.empty((sequences, heads, d, dv), dtype=torch.float32, device=v.device) if final_state else None
         if n == 0 or sequences == 0:
             if final is not None:
                 final.zero_() if initial_state is None else final.copy_(initial_state)
             return out, final, None
-        size = _abi.dism_delta_saved(starts != 0, sequences, n, heads, d, dv, bool(final_state), bool(backward))
+        size = _delta_saved_bytes(starts != 0, sequences, n, heads, d, dv, bool(final_state), bool(backward))
         saved = torch.empty((size,), dtype=torch.uint8, device=v.device)
         _lib.check(_abi.dism_delta_forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), gates_bf16,
                                            initial, starts, sequences, n, key_heads, heads, d, dv, float(scale), out.data_ptr(),
                                            final.data_ptr() if final_state else None, bool(backward), saved.data_ptr(), size,
-                                           _stream(v)))
+                                           _raw_stream(v)))
     return out, final, saved if backward else None
 
 
-def delta_backward(q, k, dout, scale, saved, gate_dtype, dfinal_state=None, initial_gradient=False, cu_seqlens=None, covered=True):
+def delta_backward(q, k, dout, scale, saved, gate_dtype, dfinal_state=None, initial_gradient=False, cu_seqlens=None):
     """Gradients of delta_forward(..., backward=True): [dq, dk bf16, dv bf16, dg, dbeta in gate_dtype, d(initial state) FP32 or None]."""
     _check(q, torch.bfloat16, None, 'q')
     _check(k, torch.bfloat16, q.shape, 'k')
@@ -559,11 +577,10 @@ def delta_backward(q, k, dout, scale, saved, gate_dtype, dfinal_state=None, init
     heads, dv = dout.shape[2:]
     sequences, starts = _delta_sequences(dout, cu_seqlens)
     dfinal = _delta_state(dfinal_state, sequences, heads, d, dv, q.device, 'final state gradient')
-    with torch.cuda.device(q.device):
-        fresh = torch.empty if covered else torch.zeros
-        dq, dk = (fresh(q.shape, dtype=q.dtype, device=q.device) for _ in range(2))
-        dvalue = fresh(dout.shape, dtype=dout.dtype, device=q.device)
-        dg, dbeta = (fresh((b, n, heads), dtype=gate_dtype, device=q.device) for _ in range(2))
+    with _on(q.device):
+        dq, dk, dvalue = torch.empty_like(q), torch.empty_like(k), torch.empty_like(dout)
+        dg = torch.empty((b, n, heads), dtype=gate_dtype, device=q.device)
+        dbeta = torch.empty_like(dg)
         dinitial = torch.empty((sequences, heads, d, dv), dtype=torch.float32, device=q.device) if initial_gradient else None
         if n == 0 or sequences == 0:
             if dinitial is not None:
@@ -571,12 +588,12 @@ def delta_backward(q, k, dout, scale, saved, gate_dtype, dfinal_state=None, init
             return [dq, dk, dvalue, dg, dbeta, dinitial]
         if not (torch.is_tensor(saved) and saved.device == q.device and saved.dtype == torch.uint8 and saved.is_contiguous()):
             _fail('saved buffer: invalid device, dtype, shape or stride')
-        size = _abi.dism_delta_backward_workspace(starts != 0, sequences, n, heads, d, dv)
+        size = _delta_workspace_bytes(starts != 0, sequences, n, heads, d, dv)
         workspace = torch.empty((size,), dtype=torch.uint8, device=q.device)
         _lib.check(_abi.dism_delta_backward(q.data_ptr(), k.data_ptr(), dout.data_ptr(), dfinal, gate_dtype == torch.bfloat16, starts,
                                             sequences, n, key_heads, heads, d, dv, float(scale), saved.data_ptr(), saved.numel(),
                                             dq.data_ptr(), dk.data_ptr(), dvalue.data_ptr(), dg.data_ptr(), dbeta.data_ptr(),
-                                            dinitial.data_ptr() if initial_gradient else None, workspace.data_ptr(), size, _stream(q)))
+                                            dinitial.data_ptr() if initial_gradient else None, workspace.data_ptr(), size, _raw_stream(q)))
     return [dq, dk, dvalue, dg, dbeta, dinitial]
 
 
@@ -597,12 +614,12 @@ def delta_step(x, scale, state, slots=None):
     elif not (torch.is_tensor(slots) and slots.device == v.device and slots.dtype == torch.int32 and tuple(slots.shape) == (batch,)
               and slots.is_contiguous()):
         _fail('slots must be contiguous int32 [B] on the operand device')
-    with torch.cuda.device(v.device):
+    with _on(v.device):
         out = torch.empty_like(v)
         if batch and state.size(0):
             _lib.check(_abi.dism_delta_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), gates_bf16,
                                             state.data_ptr(), None if slots is None else slots.data_ptr(), state.size(0), batch,
-                                            key_heads, heads, d, dv, float(scale), out.data_ptr(), _stream(v)))
+                                            key_heads, heads, d, dv, float(scale), out.data_ptr(), _raw_stream(v)))
         elif batch:
             out.zero_()
     return out
@@ -629,11 +646,11 @@ def dropout(x, residual, threshold, seed, site=0):
         _fail('the threshold must lie in 0 .. 65536')
     if not 0 <= site < 1 << 32:
         _fail('site must fit 32 bits')
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         out = torch.empty_like(x)
         if x.numel():
             _lib.check(_abi.dism_dropout(_dropout_types[x.dtype], x.data_ptr(), None if residual is None else residual.data_ptr(),
-                                         x.numel(), int(threshold), seed.data_ptr(), int(site), out.data_ptr(), _stream(x)))
+                                         x.numel(), int(threshold), seed.data_ptr(), int(site), out.data_ptr(), _raw_stream(x)))
     return out
 
 

@@ -11,34 +11,46 @@ import cu_flash_dism as cu
 
 def _ready(t):
     """Contiguous and 16-byte aligned, as the library wants its tensors; a copy only where it is needed."""
-    t = t.detach().contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _gate_type(g, beta):
+    return g.dtype if g.dtype == beta.dtype and g.dtype in (torch.float32, torch.bfloat16) else torch.float32
+
+
+def _backward(ctx, dout, dfinal):
+    q, k, saved, starts = ctx.saved_tensors
+    if dout is None:
+        dout = torch.zeros(ctx.shape, dtype=torch.bfloat16, device=q.device)
+    types, gates, scale = ctx.settings
+    dq, dk, dv, dg, dbeta, dinitial = cu.delta_backward(q, k, _ready(dout), scale, saved, gates, None if dfinal is None else _ready(dfinal),
+                                                        ctx.needs_input_grad[5], starts)
+    return (dq, dk, dv, dg if gates is types[0] else dg.to(types[0]), dbeta if gates is types[1] else dbeta.to(types[1]), dinitial,
+            None, None, None, None)
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 class _GatedDelta(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, g, beta, initial_state, scale, final_state, starts, covered, needed):
-        gates = g.dtype if g.dtype == beta.dtype and g.dtype in (torch.float32, torch.bfloat16) else torch.float32
-        initial = None if initial_state is None else _ready(initial_state)
+    def forward(ctx, q, k, v, g, beta, initial_state, scale, final_state, starts, needed):
+        gates = _gate_type(g, beta)
         ready_q, ready_k = _ready(q), _ready(k)
         out, final, saved = cu.delta_forward((ready_q, ready_k, _ready(v), _ready(g.to(gates)), _ready(beta.to(gates))), scale,
-                                             initial, final_state, starts, covered, needed)
+                                             None if initial_state is None else _ready(initial_state), final_state, starts, needed)
         if needed:
             ctx.save_for_backward(ready_q, ready_k, saved, starts)
-            ctx.types, ctx.gates, ctx.scale, ctx.covered = (g.dtype, beta.dtype), gates, scale, covered
-            ctx.set_materialize_grads(False)
+            ctx.settings = (g.dtype, beta.dtype), gates, scale
             ctx.shape = v.shape
+            ctx.set_materialize_grads(False)
         return out, final
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dfinal):
-        q, k, saved, starts = ctx.saved_tensors
-        dout = torch.zeros(ctx.shape, dtype=torch.bfloat16, device=q.device) if dout is None else _ready(dout)
-        dfinal = None if dfinal is None else _ready(dfinal)
-        dq, dk, dv, dg, dbeta, dinitial = cu.delta_backward(q, k, dout, ctx.scale, saved, ctx.gates, dfinal, ctx.needs_input_grad[5],
-                                                            starts, ctx.covered)
-        return dq, dk, dv, dg.to(ctx.types[0]), dbeta.to(ctx.types[1]), dinitial, None, None, None, None, None
+        # the gradients are not differentiable themselves; saying so costs something and is only needed when a graph of them is built
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dout, dfinal)
 
 
 _starts = {}
@@ -56,7 +68,7 @@ def _host_starts(starts, device):
 
 
 def _documents(v, cu_seqlens, layout):
-    """Device starts of the documents and whether they are known to cover every row."""
+    """Device starts of the documents of a pack."""
     if cu_seqlens is not None and layout is not None:
         raise ValueError('provide either layout or cu_seqlens, not both')
     if layout is not None:
@@ -65,17 +77,17 @@ def _documents(v, cu_seqlens, layout):
             starts.append(starts[-1] + length)
         if v.dim() != 4 or starts[-1] != v.size(1):
             raise ValueError('layout and operands differ in length')
-        return _host_starts(starts, v.device), True
+        return _host_starts(starts, v.device)
     if cu_seqlens is None:
-        return None, True
+        return None
     if not (torch.is_tensor(cu_seqlens) and cu_seqlens.dim() == 1 and cu_seqlens.dtype == torch.int32 and cu_seqlens.numel() > 1):
         raise RuntimeError('cu_seqlens must be int32 [sequences+1]')
     if cu_seqlens.device.type == 'cpu':
         starts = cu_seqlens.tolist()
         if v.dim() != 4 or starts[0] != 0 or starts[-1] != v.size(1) or any(a > b for a, b in zip(starts, starts[1:])):
             raise RuntimeError('invalid cu_seqlens: starts at 0, ascending, ends at the number of positions')
-        return _host_starts(starts, v.device), True
-    return cu_seqlens.contiguous(), False
+        return _host_starts(starts, v.device)
+    return cu_seqlens.contiguous()
 
 
 def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, output_final_state=False, cu_seqlens=None, layout=None):
@@ -90,10 +102,10 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, output
     [sequences,H,D,DV].  All operands and the initial state are differentiable; gates receive gradients in their own type, with
     the relative accuracy of the bf16 operands.  Keeping the states for a backward takes 2 D DV / 64 + 2 DV + 276 bytes per position
     and head."""
-    starts, covered = _documents(v, cu_seqlens, layout)
+    starts = _documents(v, cu_seqlens, layout)
     needed = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
     out, final = _GatedDelta.apply(q, k, v, g, beta, initial_state, q.size(-1) ** -.5 if scale is None else float(scale),
-                                   bool(output_final_state), starts, covered, needed)
+                                   bool(output_final_state), starts, needed)
     return (out, final) if output_final_state else out
 
 
@@ -104,6 +116,6 @@ def gated_delta_step(q, k, v, g, beta, state, *, scale=None, slots=None):
     `state` is FP32 [pool,H,D,DV], contiguous, and is updated in place.  `slots`, int32 [B] on the GPU, names the state of each
     row (default: state i for row i); a slot outside the pool marks a padding row, whose output is zero, and rows that name
     one slot are consecutive tokens of that sequence, in row order.  Everything is computed in 32 bits; not differentiable."""
-    gates = g.dtype if g.dtype == beta.dtype and g.dtype in (torch.float32, torch.bfloat16) else torch.float32
+    gates = _gate_type(g, beta)
     return cu.delta_step((_ready(q), _ready(k), _ready(v), _ready(g.to(gates)), _ready(beta.to(gates))),
                          q.size(-1) ** -.5 if scale is None else float(scale), state, slots)

@@ -7,14 +7,16 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, threshold, seed, site):
         ctx.save_for_backward(seed)
-        ctx.threshold, ctx.site, ctx.types = threshold, site, (x.dtype, None if residual is None else residual.dtype)
-        return cu.dropout(x.detach().contiguous(), None if residual is None else residual.detach().contiguous(), threshold, seed, site)
+        ctx.settings = threshold, site
+        return cu.dropout(x.contiguous(), None if residual is None else residual.contiguous(), threshold, seed, site)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         seed, = ctx.saved_tensors
-        dx = cu.dropout(dy.contiguous(), None, ctx.threshold, seed, ctx.site) if ctx.needs_input_grad[0] else None
+        threshold, site = ctx.settings
+        dx = None
+        if ctx.needs_input_grad[0]:  # linear in dy: under create_graph the same operator again
+            dx = _Dropout.apply(dy, None, threshold, seed, site) if torch.is_grad_enabled() else cu.dropout(dy.contiguous(), None, threshold, seed, site)
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
 
 

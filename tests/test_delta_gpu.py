@@ -104,6 +104,13 @@ def test_packed_documents(flash, starts):
     check(flash, len(starts), 1, starts[-1], 2, 4, 32, 64, starts=starts, states=True)
 
 
+@pytest.mark.parametrize('d,dv,starts', [(64, 64, None), (128, 64, None), (64, 128, [0, 1700, 1701, 1701, 2100]), (128, 128, [0, 600, 1750])])
+def test_long_chains_are_cut_into_segments(flash, d, dv, starts):
+    """Few heads and many chunks: the segments' transition matrices carry the state, and its gradient, from one to the next.  The state at
+    a segment's start has one rounding more (M), which the bounds of the shorter cases leave room for."""
+    check(flash, d + dv, 1, 2100 if starts is None else starts[-1], 1, 2, d, dv, starts=starts, states=True, decay=.02)
+
+
 @pytest.mark.parametrize('decay', [0., .01, 4.])
 def test_decays(flash, decay):
     check(flash, 7, 1, 320, 1, 2, 128, 64, states=True, decay=decay)
