@@ -121,7 +121,7 @@ struct DeltaLayout {
         int64_t first;
         int length, sequence;
         if (!cu) {
-            sequence = int(slot / chunks());
+            sequence = int(unsigned(slot) / unsigned(chunks()));  // slots fit 31 bits
         } else {
             int lo = 0, hi = sequences - 1;
             while (lo < hi) {
@@ -158,8 +158,8 @@ struct DeltaSegments {
         if (!length) {
             sequence = int(segment);
         } else if (!layout.cu) {
-            const int each = (layout.chunks() + length - 1) / length;
-            sequence = int(segment / each), number = int(segment % each);
+            const unsigned each = (layout.chunks() + length - 1) / length;
+            sequence = int(unsigned(segment) / each), number = int(unsigned(segment) % each);
         } else {
             int lo = 0, hi = layout.sequences - 1;
             while (lo < hi) {

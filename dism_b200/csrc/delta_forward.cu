@@ -8,7 +8,6 @@
 // EXACT: the state is wanted at the end.  S0 in S0 K^T, Y, T and U are then kept as bf16 pairs (value and remainder, 16 bits),
 // which holds the state to a few 1e-6; without it a single bf16 is enough for outputs that are bf16 themselves.
 #include "delta_common.cuh"
-#include <cstdlib>
 
 namespace dism {
 namespace {
@@ -348,14 +347,17 @@ cudaError_t by_width(const DeltaShape& shape, const __nv_bfloat16* q, const __nv
 }
 }  // namespace
 
+// A segment costs two CTA walks forward (one of them for B and M, without outputs) and two backward, so cutting pays when the walks
+// get at least four times shorter; with segments of equal length for two CTAs per SM (what the chains' registers and shared memory
+// allow), but no shorter than eight chunks, below which putting the starts together costs what it saves.  Measured, forward and
+// backward chain, uncut / for one / for two CTAs per SM (us): 2 x 8192, 16 heads of 64: 426 / 281 / 211; prompt of 16384, 16 heads of
+// 128: 761 / 523 / 439; pack of 7019, 8 heads: 166 / 152 / 120.  4 x 2048, 10 heads of 128 (32 chunks to 9): 204 / - / 212.
 int delta_segment_length(const DeltaLayout& layout, int heads, int d, int dv) {
     if (d < 64 || dv < 64) return 0;
-    static const int least = getenv("DELTA_LEAST") ? atoi(getenv("DELTA_LEAST")) : 8, ratio = getenv("DELTA_RATIO") ? atoi(getenv("DELTA_RATIO")) : 3;
-    static const double scale = getenv("DELTA_SCALE") ? atof(getenv("DELTA_SCALE")) : 1.;
-    const int sms = device_sm_count();
-    const int64_t chains = int64_t(heads) * (dv / 64), even = sms > 0 ? int64_t(scale * double(layout.slots() * chains + sms - 1) / sms) : 1 << 30;
-    const int64_t length = even < least ? least : even;
-    return ratio * length <= layout.chunks() ? int(length) : 0;
+    const int64_t chains = int64_t(heads) * (dv / 64), room = 2 * int64_t(device_sm_count());
+    if (room <= 0) return 0;
+    const int64_t even = (layout.slots() * chains + room - 1) / room, length = even < 8 ? 8 : even;
+    return 4 * length <= layout.chunks() ? int(length) : 0;
 }
 
 cudaError_t launch_delta_chain(const DeltaShape& shape, const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v,

@@ -49,7 +49,7 @@ __device__ __forceinline__ void load_stack(unsigned tile, const char* global, in
     const int first = thread / PIECES, piece = thread % PIECES;
     const unsigned to = tile + (piece >> 3) * STACK + first * 128;
     const char* from = global + first * stride + piece * 16;
-#pragma unroll
+#pragma unroll 1
     for (int row = 0; row < CHUNK; row += STEP) {
         const bool inside = first + row < count;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + row * 128 + (((piece & 7) ^ ((first + row) & 7)) * 16)),
@@ -57,21 +57,27 @@ __device__ __forceinline__ void load_stack(unsigned tile, const char* global, in
         from += STEP * stride;
     }
 }
-// v[i] of every lane is summed over the warp for each i; lane l keeps the sum of i = l
-__device__ __forceinline__ float transposing_sum(float (&v)[32], int lane) {
+__device__ __forceinline__ void factors(float (&f)[16], const float* from) {
 #pragma unroll
-    for (int step = 16; step; step >>= 1) {
-        const bool upper = lane & step;
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(f + 4 * i) = reinterpret_cast<const float4*>(from)[i];
+}
+// v[i] of every lane is summed over the warp for each i; lane l is left with the sum of i = l / 2
+__device__ __forceinline__ float transposing_sum(float (&v)[16], int lane) {
+#pragma unroll
+    for (int step = 8; step; step >>= 1) {
+        const bool upper = lane & (2 * step);
 #pragma unroll
         for (int i = 0; i < step; ++i) {
             const float kept = upper ? v[i + step] : v[i], sent = upper ? v[i] : v[i + step];
-            v[i] = kept + __shfl_xor_sync(FULL, sent, step);
+            v[i] = kept + __shfl_xor_sync(FULL, sent, 2 * step);
         }
     }
-    return v[0];
+    return v[0] + __shfl_xor_sync(FULL, v[0], 1);
 }
 
-template <int D, int DV>
+// SHARED: several value heads read a key head, whose gradients are summed in registers.  The loops over columns are rolled where
+// registers allow it: the loop over the items has to stay in the instruction cache (unrolled, at 62 KB, it ran at 17 000 clocks an item).
+template <int D, int DV, bool SHARED>
 __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_kernel(DeltaShape shape, const __nv_bfloat16* __restrict__ q,
                                                                                     const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ dout,
                                                                                     const __nv_bfloat16* __restrict__ dy, DeltaSaved saved,
@@ -84,20 +90,13 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
     unsigned char* shared = shared_raw + ((1024 - (tm_address(shared_raw) & 1023)) & 1023);
     __shared__ GradientControl control;
     const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31, group = shape.heads / shape.key_heads;
-    const int64_t units = shape.layout.slots() * shape.key_heads;
-    int64_t row = 0, next_row = 0, unit = blockIdx.x, next_unit;
+    // a unit is a (slot, key head); the CTA takes every gridDim.x-th
+    const int slots = int(shape.layout.slots()), step_slots = gridDim.x / shape.key_heads, step_heads = gridDim.x % shape.key_heads;
+    int slot = 0, key_head = 0, next_slot = blockIdx.x / shape.key_heads, next_key_head = blockIdx.x % shape.key_heads;
+    int64_t row = 0, next_row = 0;
     int count = 0, next_count = 0;
     if (shape.layout.cu) clear_gradients<GRADIENT_THREADS>(shape, dq, dk, dg, dbeta, blockIdx.x, gridDim.x, thread);
-    // the first unit from `from` on that has positions
-    auto find = [&](int64_t from, int64_t& at, int& positions) {
-        for (; from < units; from += gridDim.x) {
-            shape.layout.chunk(from / shape.key_heads, at, positions);
-            if (positions > 0) break;
-        }
-        return from;
-    };
-    unit = find(unit, row, count);
-    if (unit >= units) return;
+    if (next_slot >= slots) return;
     const uint32_t base = tm_address(shared);
     float* sums = reinterpret_cast<float*>(shared + Tiles::SUMS);
     const int64_t key_stride = int64_t(shape.key_heads) * D * 2, value_stride = int64_t(shape.heads) * DV * 2;
@@ -114,9 +113,9 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
     const uint32_t tensor = control.tensor_memory, lanes = tensor + (uint32_t((warp & 3) * 32) << 16);
 
     // an item's loads; `item` counts the CTA's items, `keys` is the buffer of Q and K, filled for the first head of a unit
-    auto load = [&](int64_t of_unit, int64_t at, int positions, int turn, int item, int keys) {
-        const int key_head = int(of_unit % shape.key_heads), head = key_head * group + turn;
-        const int64_t place = of_unit / shape.key_heads * shape.heads + head;
+    auto load = [&](int of_slot, int of_key_head, int64_t at, int positions, int turn, int item, int keys) {
+        const int head = of_key_head * group + turn;
+        const int64_t place = int64_t(of_slot) * shape.heads + head;
         if (thread == 0) {
             tm_expect(&control.loaded, DV * 128 + 2 * Tiles::STATE);
             tm_copy(base + Tiles::X, saved.x + place * CHUNK * DV, DV * 128, &control.loaded);
@@ -128,7 +127,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
         load_stack<DV, STACK>(base + Tiles::GRAD + HALF, reinterpret_cast<const char*>(dy) + value, value_stride, positions, thread);
         load_block<ROW_VALUES * 4, GRADIENT_THREADS>(base + Tiles::ROWS + (item & 1) * ROW_VALUES * 4, reinterpret_cast<const char*>(saved.rows + place * ROW_VALUES), thread);
         if (turn == 0) {
-            const int64_t key = (at * shape.key_heads + key_head) * D * 2;
+            const int64_t key = (at * shape.key_heads + of_key_head) * D * 2;
             const uint32_t to = base + Tiles::QK + keys * (D / 64 * STACK);
             load_stack<D, STACK>(to, reinterpret_cast<const char*>(q) + key, key_stride, positions, thread);
             load_stack<D, STACK>(to + HALF, reinterpret_cast<const char*>(k) + key, key_stride, positions, thread);
@@ -138,90 +137,106 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
 
     // this thread's row of tensor memory: position t, a query's (part 0) or a key's (part 1); its half of the columns
     const int r = thread & 127, t = r & 63, part = r >> 6, half = warp >> 2;
-    float acc[COLUMNS];  // half a row of dQ or dK
+    float acc[SHARED ? COLUMNS : 16];  // half a row of dQ or dK
 #pragma unroll
-    for (int i = 0; i < COLUMNS; ++i) acc[i] = 0.f;
-    load(unit, row, count, 0, 0, 0);
-    for (int item = 0, turn = 0, keys = 0;; ++item) {
-        const int key_head = int(unit % shape.key_heads), head = key_head * group + turn;
-        const int64_t place = unit / shape.key_heads * shape.heads + head;
+    for (int i = 0; i < COLUMNS && SHARED; ++i) acc[i] = 0.f;
+    // Turn -1 only loads the first item: one place in the code for what comes next keeps the loop's instructions few.
+    for (int item = -1, turn = 0, keys = 1;; ++item) {
+        const int head = key_head * group + turn;
+        const int64_t place = int64_t(slot) * shape.heads + head;
         const uint32_t parity = item & 1, qk_tile = base + Tiles::QK + keys * (D / 64 * STACK);
         const float* rows = reinterpret_cast<const float*>(shared + Tiles::ROWS + (item & 1) * ROW_VALUES * 4);
+        const uint64_t keys_across = tm_descriptor(qk_tile + HALF, STACK);
+        float beta_parts[DV / 16];
+        bool same_unit = false;
+        if (item >= 0) {
         cp_async_wait<0>();
         tm_fence_proxy();  // written through the generic proxy, read by the tensor cores
         tm_wait(&control.loaded, parity, abort, &delta_gradient_fault, 3);
         __syncthreads();
         tm_fence_after();
-        const uint64_t keys_across = tm_descriptor(qk_tile + HALF, STACK);
         if (warp == 0 && !*abort) {
             if (elect_one()) {
                 const uint64_t grads = tm_descriptor(base + Tiles::GRAD), x = tm_block_descriptor(base + Tiles::X, 128, CHUNK * 16);
                 const uint64_t queries = tm_descriptor(qk_tile), own_keys = tm_descriptor(qk_tile + HALF);
                 const uint64_t s0 = tm_block_descriptor(base + Tiles::S0, 128, D * 16), ds = tm_block_descriptor(base + Tiles::DS, 128, D * 16);
-#pragma unroll
+#pragma unroll 2
                 for (int kb = 0; kb < DV / 16; ++kb)
                     tm_mma_shared(tensor + TM_Z, grads + ((kb >> 2) * STACK + (kb & 3) * 32) / 16, x + kb * CHUNK * 2, tm_instruction(CHUNK, false, true), kb > 0);
-#pragma unroll
+#pragma unroll 2
                 for (int kb = 0; kb < D / 16; ++kb)
                     tm_mma_shared(tensor + TM_QK, queries + ((kb >> 2) * STACK + (kb & 3) * 32) / 16, own_keys + ((kb >> 2) * STACK + (kb & 3) * 32) / 16,
                                   tm_instruction(CHUNK, false, false), kb > 0);
-#pragma unroll
+#pragma unroll 2
                 for (int kb = 0; kb < DV / 16; ++kb)
                     tm_mma_shared(tensor + TM_U1, grads + ((kb >> 2) * STACK + (kb & 3) * 32) / 16, s0 + kb * D * 2, tm_instruction(D, false, true), kb > 0);
                 // X as rows 64-127: eight blocks before it begins
-#pragma unroll
+#pragma unroll 2
                 for (int kb = 0; kb < DV / 16; ++kb)
                     tm_mma_shared(tensor + TM_V1, x - 1024 / 16 + kb * CHUNK * 2, ds + kb * D * 2, tm_instruction(D, true, true), kb > 0);
-#pragma unroll
+#pragma unroll 2
                 for (int kb = 0; kb < DV / 16; ++kb)
                     tm_mma_shared(tensor + TM_TRACE, s0 + kb * D * 2, ds + kb * D * 2, tm_instruction(D, true, true), kb > 0);
                 tm_commit(&control.first);
             }
             __syncwarp();
         }
-        float beta_part = 0.f;  // what the reverse chain left of db
-        if (thread < CHUNK) {
+        if (thread < CHUNK) {  // what the reverse chain left of db
             const int64_t stride = shape.layout.slots() * shape.heads * CHUNK;
 #pragma unroll
-            for (int i = 0; i < DV / 16; ++i) beta_part += __ldg(dbeta_parts + i * stride + place * CHUNK + thread);
+            for (int i = 0; i < DV / 16; ++i) beta_parts[i] = __ldg(dbeta_parts + i * stride + place * CHUNK + thread);
         }
-        const bool same_unit = turn + 1 < group;
-        next_unit = same_unit ? unit : find(unit + gridDim.x, next_row, next_count);
-        if (same_unit) next_row = row, next_count = count;
+        same_unit = turn + 1 < group;
         tm_wait(&control.first, parity, abort, &delta_gradient_fault, 1);
         tm_fence_after();
-        if (next_unit < units) load(next_unit, next_row, next_count, same_unit ? turn + 1 : 0, item + 1, same_unit ? keys : keys ^ 1);
+        }
+        if (!same_unit) {
+            auto advance = [&]() {
+                next_slot += step_slots, next_key_head += step_heads;
+                if (next_key_head >= shape.key_heads) next_key_head -= shape.key_heads, ++next_slot;
+            };
+            if (item >= 0) advance();
+            for (; next_slot < slots; advance()) {
+                shape.layout.chunk(next_slot, next_row, next_count);
+                if (next_count > 0) break;
+            }
+        }
+        if (next_slot < slots) load(next_slot, next_key_head, next_row, next_count, same_unit ? turn + 1 : 0, item + 1, same_unit ? keys : keys ^ 1);
+        if (item >= 0) {
         // dP~ or dL~ of this row: columns 32 half .. 32 half + 31
         {
             const float high = rows[ROW_HIGH + t], low = rows[ROW_LOW + t];
-            float w[32], row_sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; j += 16) {
+            float row_sum = 0.f;
+#pragma unroll 1
+            for (int j = 32 * half; j < 32 * half + 32; j += 16) {
                 float z[16], y[16];
-                tm_load16(z, lanes + TM_Z + 32 * half + j);
-                tm_load16(y, lanes + TM_QK + 32 * half + j);
+                tm_load16(z, lanes + TM_Z + j);
+                tm_load16(y, lanes + TM_QK + j);
+                float h[16], l[16], beta[16];
+                factors(h, rows + ROW_HIGH + j);
+                factors(l, rows + ROW_LOW + j);
+                factors(beta, rows + ROW_BETA + j);
                 tm_wait_load();
-                float d[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int s = 32 * half + j + i;
-                    const float between = ex2((high - rows[ROW_HIGH + s]) + (low - rows[ROW_LOW + s]));
-                    const bool counts = s + part <= t;  // s <= t for queries, s < t for keys
+                    const float between = ex2((high - h[i]) + (low - l[i]));
+                    const bool counts = j + i + part <= t;  // s <= t for queries, s < t for keys
                     const float x = counts ? (part ? -between : shape.scale * between) * z[i] : 0.f;
-                    d[i] = x * rows[ROW_BETA + s];
-                    w[j + i] = x * y[i];
-                    row_sum += __fmul_rn(rows[ROW_BETA + s], w[j + i]);  // as the column sums have it: a pair that cancels in dG is one number
+                    z[i] = x * beta[i];
+                    y[i] *= x;
+                    row_sum += __fmul_rn(beta[i], y[i]);  // as the column sums have it: a pair that cancels in dG is one number
                 }
 #pragma unroll
                 for (int i = 0; i < 16; i += 8)
-                    *reinterpret_cast<uint4*>(shared + Tiles::PAIRS + r * 128 + (((4 * half + (j + i) / 8) ^ (r & 7)) * 16)) =
-                        make_uint4(pack2(d[i], d[i + 1]), pack2(d[i + 2], d[i + 3]), pack2(d[i + 4], d[i + 5]), pack2(d[i + 6], d[i + 7]));
+                    *reinterpret_cast<uint4*>(shared + Tiles::PAIRS + r * 128 + ((((j + i) / 8) ^ (r & 7)) * 16)) =
+                        make_uint4(pack2(z[i], z[i + 1]), pack2(z[i + 2], z[i + 3]), pack2(z[i + 4], z[i + 5]), pack2(z[i + 6], z[i + 7]));
+                const float column = transposing_sum(y, lane);
+                if (!(lane & 1)) sums[Tiles::COLUMN_SUM + (warp & 3) * CHUNK + j + lane / 2] = column;
             }
             sums[Tiles::ROW_SUM + half * 128 + r] = row_sum;
-            sums[Tiles::COLUMN_SUM + (warp & 3) * CHUNK + 32 * half + lane] = transposing_sum(w, lane);
             if (half == 0 && r < D) {  // the trace: element r of this row
                 float dot = 0.f;
-#pragma unroll
+#pragma unroll 1
                 for (int j = 0; j < 32; j += 16) {
                     float x[16];
                     tm_load16(x, lanes + TM_TRACE + (warp & 3) * 32 + j);
@@ -233,7 +248,12 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                 for (int m = 16; m; m >>= 1) dot += __shfl_xor_sync(FULL, dot, m);
                 if (lane == 0) sums[Tiles::DOT + warp] = dot;
             }
-            if (thread < CHUNK) sums[Tiles::BETA + thread] = beta_part;
+            if (thread < CHUNK) {
+                float beta_part = 0.f;
+#pragma unroll
+                for (int i = 0; i < DV / 16; ++i) beta_part += beta_parts[i];
+                sums[Tiles::BETA + thread] = beta_part;
+            }
         }
         tm_fence_proxy();
         tm_fence_before();
@@ -243,13 +263,13 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
             if (elect_one()) {
                 const uint64_t pairs = tm_descriptor(base + Tiles::PAIRS), p_across = tm_descriptor(base + Tiles::PAIRS, 0), l_across = tm_descriptor(base + Tiles::PAIRS + HALF, 0);
                 const uint64_t queries_across = tm_descriptor(qk_tile, STACK);
-#pragma unroll
+#pragma unroll 2
                 for (int kb = 0; kb < CHUNK / 16; ++kb)
                     tm_mma_shared(tensor + TM_U2, pairs + kb * 32 / 16, keys_across + kb * 2048 / 16, tm_instruction(D, false, true), kb > 0);
-#pragma unroll
+#pragma unroll 2
                 for (int kb = 0; kb < CHUNK / 16; ++kb)
                     tm_mma_shared(tensor + TM_V2, l_across + kb * 2048 / 16, keys_across + kb * 2048 / 16, tm_instruction(D, true, true), kb > 0);
-#pragma unroll
+#pragma unroll 2
                 for (int kb = 0; kb < CHUNK / 16; ++kb)
                     tm_mma_shared(tensor + TM_V2, p_across + kb * 2048 / 16, queries_across + kb * 2048 / 16, tm_instruction(D, true, true), true);
                 tm_commit(&control.second);
@@ -262,8 +282,8 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
             const float decay = rows[ROW_DECAY + t], f1 = part ? -decay : shape.scale * decay, f2 = rows[ROW_WRITE + t];
             float state_sum = 0.f, last_sum = 0.f;
             const unsigned char* own = shared + Tiles::QK + keys * (D / 64 * STACK) + (half * COLUMNS >> 6) * STACK + r * 128;  // the row of Q or K
-#pragma unroll
-            for (int j = 0; j < COLUMNS; j += 16) {
+            __nv_bfloat16* to = (part ? dk : dq) + ((row + t) * shape.key_heads + key_head) * D + half * COLUMNS;
+            auto take = [&](int j, float* sum) {  // sixteen columns
                 const int column = half * COLUMNS + j;
                 float u1[16], u2[16], v1[16], v2[16];
                 tm_load16(u1, lanes + TM_U1 + column);
@@ -281,12 +301,32 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                     const float own_value = i & 1 ? high_half(x[i / 2]) : low_half(x[i / 2]);
                     const float a = f1 * u1[i];
                     state_sum += a * own_value;
-                    acc[j + i] += a + u2[i];
+                    sum[i] += a + u2[i];
                     if (part) {
                         const float b = f2 * v1[i];
                         last_sum += b * own_value;
-                        acc[j + i] += b + v2[i];
+                        sum[i] += b + v2[i];
                     }
+                }
+            };
+            auto store = [&](int j, const float* sum) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 8)
+                    *reinterpret_cast<uint4*>(to + j + i) = make_uint4(pack2(sum[i], sum[i + 1]), pack2(sum[i + 2], sum[i + 3]), pack2(sum[i + 4], sum[i + 5]), pack2(sum[i + 6], sum[i + 7]));
+            };
+            if constexpr (SHARED) {
+#pragma unroll
+                for (int j = 0; j < COLUMNS; j += 16) {
+                    take(j, acc + j);
+                    if (!same_unit && t < count) store(j, acc + j);
+                }
+            } else {
+#pragma unroll 1
+                for (int j = 0; j < COLUMNS; j += 16) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+                    take(j, acc);
+                    if (t < count) store(j, acc);
                 }
             }
             sums[Tiles::STATE_SUM + half * 128 + r] = state_sum;
@@ -342,20 +382,15 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                 }
             }
         }
+        }
+        if (next_slot >= slots) break;
         if (!same_unit) {
-            if (t < count) {
-                __nv_bfloat16* to = (part ? dk : dq) + ((row + t) * shape.key_heads + key_head) * D + half * COLUMNS;
 #pragma unroll
-                for (int i = 0; i < COLUMNS; i += 8)
-                    *reinterpret_cast<uint4*>(to + i) = make_uint4(pack2(acc[i], acc[i + 1]), pack2(acc[i + 2], acc[i + 3]), pack2(acc[i + 4], acc[i + 5]), pack2(acc[i + 6], acc[i + 7]));
-            }
-            if (next_unit >= units) break;
-#pragma unroll
-            for (int i = 0; i < COLUMNS; ++i) acc[i] = 0.f;
+            for (int i = 0; i < COLUMNS && SHARED; ++i) acc[i] = 0.f;
             keys ^= 1;
         }
         turn = same_unit ? turn + 1 : 0;
-        unit = next_unit, row = next_row, count = next_count;
+        slot = next_slot, key_head = next_key_head, row = next_row, count = next_count;
     }
     __syncthreads();
     if (control.abort) __nanosleep(1000000);  // copies and products in flight end before their memory is given back
@@ -365,10 +400,10 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
     }
 }
 
-template <int D, int DV>
+template <int D, int DV, bool SHARED>
 cudaError_t launch(const DeltaShape& shape, const DeltaGradients& x, const DeltaSaved& saved, cudaStream_t stream) {
     constexpr int BYTES = GradientTiles<D, DV>::BYTES;
-    constexpr auto* kernel = delta_gradient_tensor_kernel<D, DV>;
+    constexpr auto* kernel = delta_gradient_tensor_kernel<D, DV, SHARED>;
     if (cudaError_t status = allow_shared<kernel>(BYTES)) return status;
     KernelTimer timer("delta_gradient", stream);
     const int64_t units = shape.layout.slots() * shape.key_heads;
@@ -376,11 +411,15 @@ cudaError_t launch(const DeltaShape& shape, const DeltaGradients& x, const Delta
         shape, x.q, x.k, x.dout, x.dv, saved, x.dstates, x.dbeta_parts, x.dq, x.dk, x.dg, x.dbeta);
     return cudaGetLastError();
 }
+template <int D, int DV>
+cudaError_t choose(const DeltaShape& shape, const DeltaGradients& x, const DeltaSaved& saved, cudaStream_t stream) {
+    return shape.heads > shape.key_heads ? launch<D, DV, true>(shape, x, saved, stream) : launch<D, DV, false>(shape, x, saved, stream);
+}
 }  // namespace
 
 cudaError_t launch_delta_gradient_tensor(const DeltaShape& shape, const DeltaGradients& x, const DeltaSaved& saved, cudaStream_t stream) {
-    if (shape.d == 64) return shape.dv == 64 ? launch<64, 64>(shape, x, saved, stream) : launch<64, 128>(shape, x, saved, stream);
-    return shape.dv == 64 ? launch<128, 64>(shape, x, saved, stream) : launch<128, 128>(shape, x, saved, stream);
+    if (shape.d == 64) return shape.dv == 64 ? choose<64, 64>(shape, x, saved, stream) : choose<64, 128>(shape, x, saved, stream);
+    return shape.dv == 64 ? choose<128, 64>(shape, x, saved, stream) : choose<128, 128>(shape, x, saved, stream);
 }
 
 cudaError_t read_delta_fault(int* code) {
