@@ -30,7 +30,8 @@ template <int D, int DV>
 struct GradientTiles {
     static constexpr int STACK = 128 * 128;  // bytes of 128 rows by 64 columns
     static constexpr int STATE = 2 * D * DV;
-    static constexpr int QK = 0, GRAD = QK + 2 * (D / 64) * STACK, PAIRS = GRAD + DV / 64 * STACK, X = PAIRS + STACK, S0 = X + DV * 128, DS = S0 + STATE;
+    // the room of the pairs is also that of dQ and dK on their way out: 32 rows by half of D for each of the eight warps
+    static constexpr int QK = 0, GRAD = QK + 2 * (D / 64) * STACK, PAIRS = GRAD + DV / 64 * STACK, X = PAIRS + D / 64 * STACK, S0 = X + DV * 128, DS = S0 + STATE;
     static constexpr int ROWS = DS + STATE, SUMS = ROWS + 2 * ROW_VALUES * 4;
     // floats: rows of M [2][128], columns of M / b [4][64], state terms of dG [2][128], of dG_63 [2][64], <dS1, S0> [4], the part of db from dU [64]
     static constexpr int ROW_SUM = 0, COLUMN_SUM = 256, STATE_SUM = COLUMN_SUM + 256, LAST_SUM = STATE_SUM + 256, DOT = LAST_SUM + 128, BETA = DOT + 4;
@@ -282,7 +283,8 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
             const float decay = rows[ROW_DECAY + t], f1 = part ? -decay : shape.scale * decay, f2 = rows[ROW_WRITE + t];
             float state_sum = 0.f, last_sum = 0.f;
             const unsigned char* own = shared + Tiles::QK + keys * (D / 64 * STACK) + (half * COLUMNS >> 6) * STACK + r * 128;  // the row of Q or K
-            __nv_bfloat16* to = (part ? dk : dq) + ((row + t) * shape.key_heads + key_head) * D + half * COLUMNS;
+            constexpr int ROW = 2 * COLUMNS, PIECES = ROW / 16;
+            unsigned char* stage = shared + Tiles::PAIRS + warp * 32 * ROW;
             auto take = [&](int j, float* sum) {  // sixteen columns
                 const int column = half * COLUMNS + j;
                 float u1[16], u2[16], v1[16], v2[16];
@@ -312,13 +314,13 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
             auto store = [&](int j, const float* sum) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 8)
-                    *reinterpret_cast<uint4*>(to + j + i) = make_uint4(pack2(sum[i], sum[i + 1]), pack2(sum[i + 2], sum[i + 3]), pack2(sum[i + 4], sum[i + 5]), pack2(sum[i + 6], sum[i + 7]));
+                    *reinterpret_cast<uint4*>(stage + lane * ROW + (((j + i) / 8 ^ piece_key<ROW>(lane)) * 16)) = make_uint4(pack2(sum[i], sum[i + 1]), pack2(sum[i + 2], sum[i + 3]), pack2(sum[i + 4], sum[i + 5]), pack2(sum[i + 6], sum[i + 7]));
             };
             if constexpr (SHARED) {
 #pragma unroll
                 for (int j = 0; j < COLUMNS; j += 16) {
                     take(j, acc + j);
-                    if (!same_unit && t < count) store(j, acc + j);
+                    if (!same_unit) store(j, acc + j);
                 }
             } else {
 #pragma unroll 1
@@ -326,7 +328,18 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
 #pragma unroll
                     for (int i = 0; i < 16; ++i) acc[i] = 0.f;
                     take(j, acc);
-                    if (t < count) store(j, acc);
+                    store(j, acc);
+                }
+            }
+            if (!same_unit) {  // whole lines: a thread's own row, piece by piece, would cost the load-store unit a line per lane
+                __syncwarp();
+                const int first = (warp & 1) * 32;
+                __nv_bfloat16* to = (part ? dk : dq) + ((row + first) * shape.key_heads + key_head) * D + half * COLUMNS;
+#pragma unroll 2
+                for (int i = lane; i < 32 * PIECES; i += 32) {
+                    const int line = i / PIECES, piece = i % PIECES;
+                    const uint4 x = *reinterpret_cast<const uint4*>(stage + line * ROW + ((piece ^ piece_key<ROW>(line)) * 16));
+                    if (first + line < count) *reinterpret_cast<uint4*>(to + int64_t(line) * shape.key_heads * D + piece * 8) = x;
                 }
             }
             sums[Tiles::STATE_SUM + half * 128 + r] = state_sum;
