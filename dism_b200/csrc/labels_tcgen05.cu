@@ -36,6 +36,7 @@
 #include <cuda.h>
 
 #include "dism_common.cuh"
+#include "tensor_memory.cuh"
 
 namespace dism {
 namespace {
@@ -746,6 +747,10 @@ cudaError_t launch(const CUtensorMap (&x_map)[2], const CUtensorMap (&code_map)[
 }
 
 }  // namespace
+
+bool encode_rows(CUtensorMap* map, const void* data, uint64_t rows, uint64_t columns, uint64_t row_stride, int box_rows) {
+    return make_map(map, data, rows, columns, row_stride, box_rows);
+}
 
 bool labels_tcgen05_covers(const void* x, const void* codebook, int batch, int n, int heads, int d, int vocab) {
     return (d == 64 || d == 128) && vocab % TILE_CODES == 0 && int64_t(vocab) * d * 2 <= MAX_CODE_BYTES && shared_bytes(d, vocab) <= SHARED_LIMIT && n % TILE_ROWS == 0 &&

@@ -5,13 +5,15 @@
 // along its rows (K-major; the next sixteen are 32 bytes further, the next eight rows 1024) and with the contraction across them
 // (MN-major; the next sixteen are 2048 bytes further, the next 64 of the other index one block further).
 #pragma once
+#include <cuda.h>
+
 #include "dism_common.cuh"
 
 namespace dism {
 
 // Every wait is bounded, by about a second.  When one runs out, `abort` is set, the code is recorded and every later wait of the CTA
 // returns at once: all roles run to their ends with whatever the buffers hold, no product is issued any more, tensor memory is freed.
-constexpr unsigned TM_POLLS = 1u << 25;
+constexpr unsigned TM_WAIT_TRIES = 1u << 16, TM_PARK_NANOSECONDS = 20000;
 
 __device__ __forceinline__ uint32_t tm_address(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void tm_barrier_init(uint64_t* bar, int count) {
@@ -20,24 +22,22 @@ __device__ __forceinline__ void tm_barrier_init(uint64_t* bar, int count) {
 __device__ __forceinline__ void tm_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tm_address(bar)) : "memory");
 }
-__device__ __forceinline__ bool tm_test(uint64_t* bar, uint32_t parity) {
+// The hardware may park the warp for a while: a polling warp takes issue slots from the working ones.
+__device__ __forceinline__ bool tm_test_parked(uint64_t* bar, uint32_t parity) {
     uint32_t done;
-    asm volatile("{.reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}"
-                 : "=r"(done) : "r"(tm_address(bar)), "r"(parity) : "memory");
+    asm volatile("{.reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p;}"
+                 : "=r"(done) : "r"(tm_address(bar)), "r"(parity), "r"(TM_PARK_NANOSECONDS) : "memory");
     return done != 0;
 }
-__device__ __forceinline__ bool tm_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort, int* fault, int code) {
-    for (unsigned polls = 0; polls < TM_POLLS; ++polls) {
-        if (tm_test(bar, parity)) return true;
-        if ((polls & 255) == 255 && *abort) return false;
+// False: this wait ran out or another role's did.
+__device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* fault, int code) {
+    for (unsigned tries = 0; tries < TM_WAIT_TRIES; ++tries) {
+        if (tm_test_parked(bar, parity)) return true;
+        if (*abort) return false;
     }
     *abort = 1;
     atomicCAS(fault, 0, code);
     return false;
-}
-// False: this wait ran out or another role's did.  Polling: these waits are links of a chain, and a parked warp wakes late.
-__device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* fault, int code) {
-    return tm_test(bar, parity) || tm_wait_slow(bar, parity, abort, fault, code);
 }
 
 // Contiguous bytes (a multiple of 16, both addresses 16-byte aligned) into shared memory; the barrier counts them.
@@ -48,7 +48,15 @@ __device__ __forceinline__ void tm_copy(uint32_t to, const void* from, uint32_t 
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(to), "l"(from), "r"(bytes), "r"(tm_address(bar)) : "memory");
 }
-__device__ __forceinline__ bool elect_one() {  // one lane of a converged warp
+// A box of a tensor map, by its first column and row.
+__device__ __forceinline__ void tm_load_box(uint32_t to, const CUtensorMap* map, int column, int row, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(to), "l"(map), "r"(column), "r"(row), "r"(tm_address(bar)) : "memory");
+}
+// Tensor map of a bf16 matrix [rows, columns] (row stride in elements) in boxes of 64 columns by box_rows rows, 128-byte swizzle
+// (labels_tcgen05.cu).  False: the driver has no such entry point or refuses the shape.
+bool encode_rows(CUtensorMap* map, const void* data, uint64_t rows, uint64_t columns, uint64_t row_stride, int box_rows);
+__device__ __forceinline__ bool tm_elect() {  // one lane of a converged warp
     uint32_t elected;
     asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(elected));
     return elected != 0;
