@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
             }
         // the part of db that needs dU: this warp's 16 columns of dU.X
         float* part = dbeta_parts + (int64_t(column / 16) * shape.layout.slots() * shape.heads + place) * CHUNK;
-        unsigned dx[TILES / 2][4];
+        unsigned dx[TILES / 2][4], dx_rest[TILES / 2][4];  // a pair: its rounding would be one more in dV and in all that follows
         cp_async_wait<1>();  // all but the next chunk
         __syncwarp();
 #pragma unroll
@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
                 tile[0] *= b.x, tile[1] *= b.y, tile[2] *= b.x, tile[3] *= b.y;
             }
             to_operand(dx[np], du[2 * np], du[2 * np + 1]);
+            to_operand_rest(dx_rest[np], dx[np], du[2 * np], du[2 * np + 1]);
         }
         float(&dy)[TILES][4] = du;
 #pragma unroll
@@ -215,6 +216,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
                 ldsm4_trans(b, inverse + tile_at(kb, np));
                 mma16816(dy[2 * np], dx[kb], b[0], b[1]);
                 mma16816(dy[2 * np + 1], dx[kb], b[2], b[3]);
+                mma16816(dy[2 * np], dx_rest[kb], b[0], b[1]);
+                mma16816(dy[2 * np + 1], dx_rest[kb], b[2], b[3]);
             }
         if (!LOCAL) {
             // dV leaves through the warp's room of X: rows of 32 bytes, the halves of rows 4-7 of every eight exchanged

@@ -5,8 +5,10 @@
 // X = T Y, U = b X, O = scale e^G Q S0 + P U, S1 = e^{G_63} S0 + K^T (e^{G_63 - G} U).  Warps share K, Q, T and P of the
 // chunk in shared memory, double-buffered with cp.async; nothing else passes between them.
 //
-// EXACT: the state is wanted at the end.  S0 in S0 K^T, Y, T and U are then kept as bf16 pairs (value and remainder, 16 bits),
-// which holds the state to a few 1e-6; without it a single bf16 is enough for outputs that are bf16 themselves.
+// What is rounded: products take bf16, so every operand that is not one already is rounded, once, or kept as a pair (value and
+// remainder, 16 bits) for a second product.  Y and what is added to the state are pairs always: these roundings would reach every
+// later position (with slow decays each alone costs the gradients 2e-3 of their norm, as much as their own rounding to bf16).
+// EXACT: the state is wanted at the end.  S0 in S0 K^T and T are pairs as well then, which holds the state to a few 1e-6.
 #include "delta_common.cuh"
 
 namespace dism {
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
         }
         // Y, as the left operand of X = T Y
         const unsigned values = tile_cols_first<Stage::VALUE_PITCH>(stage + Stage::V, lane).at(warp * 32);
-        unsigned y[TILES / 2][4], y_rest[EXACT ? TILES / 2 : 1][4];
+        unsigned y[TILES / 2][4], y_rest[TILES / 2][4];
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np) {
             unsigned vv[4] = {0, 0, 0, 0};
@@ -182,7 +184,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
                 o[0] *= sx, o[1] *= sy, o[2] *= sx, o[3] *= sy;
             }
             to_operand(y[np], ks[2 * np], ks[2 * np + 1]);
-            if (EXACT) to_operand_rest(y_rest[np], y[np], ks[2 * np], ks[2 * np + 1]);
+            to_operand_rest(y_rest[np], y[np], ks[2 * np], ks[2 * np + 1]);
         }
         float(&x)[TILES][4] = ks;
 #pragma unroll
@@ -198,9 +200,9 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
                 ldsm4(b, inverse + tile_at(np, kb));
                 mma16816(x[2 * np], y[kb], b[0], b[1]);
                 mma16816(x[2 * np + 1], y[kb], b[2], b[3]);
+                mma16816(x[2 * np], y_rest[kb], b[0], b[1]);
+                mma16816(x[2 * np + 1], y_rest[kb], b[2], b[3]);
                 if (EXACT) {
-                    mma16816(x[2 * np], y_rest[kb], b[0], b[1]);
-                    mma16816(x[2 * np + 1], y_rest[kb], b[2], b[3]);
                     ldsm4(b, inverse + Stage::T_REST - Stage::T + tile_at(np, kb));
                     mma16816(x[2 * np], y[kb], b[0], b[1]);
                     mma16816(x[2 * np + 1], y[kb], b[2], b[3]);
@@ -229,7 +231,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
             for (int n = 0; n < TILES; ++n) to[n * 32] = pack2(x[n][0], x[n][1]), to[(TILES + n) * 32] = pack2(x[n][2], x[n][3]);
         }
         // U, as left operand of P U; then with the decay to the chunk's end, of the state's update
-        unsigned u[TILES / 2][4], u_rest[EXACT ? TILES / 2 : 1][4];
+        unsigned u[TILES / 2][4], u_rest[TILES / 2][4];
 #pragma unroll
         for (int np = 0; np < TILES / 2; ++np) {
 #pragma unroll
@@ -262,7 +264,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
                 tile[0] *= tail.x, tile[1] *= tail.y, tile[2] *= tail.x, tile[3] *= tail.y;
             }
             to_operand(u[np], x[2 * np], x[2 * np + 1]);
-            if (EXACT) to_operand_rest(u_rest[np], u[np], x[2 * np], x[2 * np + 1]);
+            to_operand_rest(u_rest[np], u[np], x[2 * np], x[2 * np + 1]);
         }
 #pragma unroll
         for (int n = 0; n < D / 8; ++n)
@@ -277,10 +279,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
                 ldsm4_trans(b, keys_trans.at(np * 32) + kb * 16 * Stage::PITCH);
                 mma16816(s[2 * np], u[kb], b[0], b[1]);
                 mma16816(s[2 * np + 1], u[kb], b[2], b[3]);
-                if (EXACT) {
-                    mma16816(s[2 * np], u_rest[kb], b[0], b[1]);
-                    mma16816(s[2 * np + 1], u_rest[kb], b[2], b[3]);
-                }
+                mma16816(s[2 * np], u_rest[kb], b[0], b[1]);
+                mma16816(s[2 * np + 1], u_rest[kb], b[2], b[3]);
             }
     }
     if (LOCAL) {
