@@ -152,7 +152,7 @@ struct DeltaSegments {
         if (!layout.cu) return int64_t(layout.sequences) * ((layout.chunks() + length - 1) / length);
         return layout.slots() / length + layout.sequences;
     }
-    // Sequence and number in it of a segment.
+    // Sequence and number in it of a segment; a negative number before the first document, a too large one behind a sequence's end.
     __device__ void find(const DeltaLayout& layout, int64_t segment, int& sequence, int& number) const {
         number = 0;
         if (!length) {

@@ -38,6 +38,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
     int64_t row, slot;
     int length, sequence, number;
     shape.segments.find(shape.layout, blockIdx.x, sequence, number);
+    if (number < 0) return;  // segments before the first document
     shape.layout.span(sequence, row, length, slot);
     const unsigned base = smem_address(shared);
     if (!LOCAL && shape.layout.cu && number == 0) {

@@ -489,8 +489,14 @@ def _raw_stream(tensor):
 
 
 _current_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-_delta_saved_bytes = functools.lru_cache(256)(_abi.dism_delta_saved)
-_delta_workspace_bytes = functools.lru_cache(256)(_abi.dism_delta_backward_workspace)
+@functools.lru_cache(256)
+def _delta_saved_bytes(device, *shape):  # `device` is current: how chains are cut depends on it
+    return _abi.dism_delta_saved(*shape)
+
+
+@functools.lru_cache(256)
+def _delta_workspace_bytes(device, *shape):
+    return _abi.dism_delta_backward_workspace(*shape)
 
 
 def _delta_operands(q, k, v, g, beta, tail):
@@ -555,7 +561,7 @@ def delta_forward(x, scale, initial_state=None, final_state=False, cu_seqlens=No
             if final is not None:
                 final.zero_() if initial_state is None else final.copy_(initial_state)
             return out, final, None
-        size = _delta_saved_bytes(starts != 0, sequences, n, heads, d, dv, bool(final_state), bool(backward))
+        size = _delta_saved_bytes(v.device.index, starts != 0, sequences, n, heads, d, dv, bool(final_state), bool(backward))
         saved = torch.empty((size,), dtype=torch.uint8, device=v.device)
         _lib.check(_abi.dism_delta_forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), gates_bf16,
                                            initial, starts, sequences, n, key_heads, heads, d, dv, float(scale), out.data_ptr(),
@@ -588,7 +594,7 @@ def delta_backward(q, k, dout, scale, saved, gate_dtype, dfinal_state=None, init
             return [dq, dk, dvalue, dg, dbeta, dinitial]
         if not (torch.is_tensor(saved) and saved.device == q.device and saved.dtype == torch.uint8 and saved.is_contiguous()):
             _fail('saved buffer: invalid device, dtype, shape or stride')
-        size = _delta_workspace_bytes(starts != 0, sequences, n, heads, d, dv)
+        size = _delta_workspace_bytes(q.device.index, starts != 0, sequences, n, heads, d, dv)
         workspace = torch.empty((size,), dtype=torch.uint8, device=q.device)
         _lib.check(_abi.dism_delta_backward(q.data_ptr(), k.data_ptr(), dout.data_ptr(), dfinal, gate_dtype == torch.bfloat16, starts,
                                             sequences, n, key_heads, heads, d, dv, float(scale), saved.data_ptr(), saved.numel(),

@@ -19,38 +19,50 @@ def _gate_type(g, beta):
     return g.dtype if g.dtype == beta.dtype and g.dtype in (torch.float32, torch.bfloat16) else torch.float32
 
 
-def _backward(ctx, dout, dfinal):
-    q, k, saved, starts = ctx.saved_tensors
+def _backward(ctx, dout, dfinal=None):
+    saved = ctx.saved_tensors
+    types, gates, scale, shape = ctx.settings
     if dout is None:
-        dout = torch.zeros(ctx.shape, dtype=torch.bfloat16, device=q.device)
-    types, gates, scale = ctx.settings
-    dq, dk, dv, dg, dbeta, dinitial = cu.delta_backward(q, k, _ready(dout), scale, saved, gates, None if dfinal is None else _ready(dfinal),
-                                                        ctx.needs_input_grad[5], starts)
+        dout = torch.zeros(shape, dtype=torch.bfloat16, device=saved[0].device)
+    dq, dk, dv, dg, dbeta, dinitial = cu.delta_backward(saved[0], saved[1], _ready(dout), scale, saved[2], gates, None if dfinal is None else _ready(dfinal),
+                                                        ctx.needs_input_grad[5], saved[3] if len(saved) > 3 else None)
     return (dq, dk, dv, dg if gates is types[0] else dg.to(types[0]), dbeta if gates is types[1] else dbeta.to(types[1]), dinitial,
             None, None, None, None)
 
 
-_backward_once = torch.autograd.function.once_differentiable(_backward)
+class _NotTwice(torch.autograd.Function):
+    """Hands gradients on and refuses to be differentiated, whether or not what they depend on is a part of the graph."""
+    @staticmethod
+    def forward(ctx, anchor, *grads):
+        return tuple(t.view_as(t) for t in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError('the gradients of gated_delta_rule are not differentiable')
 
 
 class _GatedDelta(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, initial_state, scale, final_state, starts, needed):
         gates = _gate_type(g, beta)
-        ready_q, ready_k = _ready(q), _ready(k)
-        out, final, saved = cu.delta_forward((ready_q, ready_k, _ready(v), _ready(g.to(gates)), _ready(beta.to(gates))), scale,
+        q, k = _ready(q), _ready(k)
+        out, final, saved = cu.delta_forward((q, k, _ready(v), _ready(g if gates is g.dtype else g.to(gates)),
+                                              _ready(beta if gates is beta.dtype else beta.to(gates))), scale,
                                              None if initial_state is None else _ready(initial_state), final_state, starts, needed)
         if needed:
-            ctx.save_for_backward(ready_q, ready_k, saved, starts)
-            ctx.settings = (g.dtype, beta.dtype), gates, scale
-            ctx.shape = v.shape
+            ctx.save_for_backward(*((q, k, saved) if starts is None else (q, k, saved, starts)))
+            ctx.settings = (g.dtype, beta.dtype), gates, scale, v.shape
             ctx.set_materialize_grads(False)
-        return out, final
+        return (out, final) if final_state else out
 
     @staticmethod
-    def backward(ctx, dout, dfinal):
-        # the gradients are not differentiable themselves; saying so costs something and is only needed when a graph of them is built
-        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dout, dfinal)
+    def backward(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return _backward(ctx, *grads)
+        with torch.no_grad():  # create_graph=True
+            result = _backward(ctx, *grads)
+        present = iter(_NotTwice.apply(torch.zeros((), requires_grad=True), *[t for t in result if t is not None]))
+        return tuple(t if t is None else next(present) for t in result)
 
 
 _starts = {}
@@ -103,10 +115,10 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, output
     the relative accuracy of the bf16 operands.  Keeping the states for a backward takes 2 D DV / 64 + 2 DV + 276 bytes per position
     and head."""
     starts = _documents(v, cu_seqlens, layout)
-    needed = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
-    out, final = _GatedDelta.apply(q, k, v, g, beta, initial_state, q.size(-1) ** -.5 if scale is None else float(scale),
+    needed = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad
+                                          or initial_state is not None and initial_state.requires_grad)
+    return _GatedDelta.apply(q, k, v, g, beta, initial_state, q.size(-1) ** -.5 if scale is None else float(scale),
                                    bool(output_final_state), starts, needed)
-    return (out, final) if output_final_state else out
 
 
 @torch.no_grad()
@@ -117,5 +129,7 @@ def gated_delta_step(q, k, v, g, beta, state, *, scale=None, slots=None):
     row (default: state i for row i); a slot outside the pool marks a padding row, whose output is zero, and rows that name
     one slot are consecutive tokens of that sequence, in row order.  Everything is computed in 32 bits; not differentiable."""
     gates = _gate_type(g, beta)
+    if torch.is_tensor(state) and not state.is_inference():
+        torch.autograd.graph.increment_version(state)  # a graph that has saved the state sees that it changes
     return cu.delta_step((_ready(q), _ready(k), _ready(v), _ready(g.to(gates)), _ready(beta.to(gates))),
                          q.size(-1) ** -.5 if scale is None else float(scale), state, slots)

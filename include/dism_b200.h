@@ -172,7 +172,7 @@ int dism_longest_match(const int32_t *streams, int batch, int n, int32_t *end, i
  * defined only for ascending ones; rows before the first and behind the last document come out as zeros.  initial_state NULL: zeros; final_state NULL: not wanted.
  * With a final state the chain of chunks carries its operands as pairs of bf16 (16 bits), without one as single bf16.
  * `saved`: dism_delta_saved bytes, 256-byte aligned; dead after the call unless `backward` is set: then dism_delta_backward
- * of the same call takes it (a size computed with final_state serves both). */
+ * of the same call takes it (a size computed with final_state serves both).  The sizes are those of the current device. */
 size_t dism_delta_saved(int packed, int sequences, int n, int heads, int d, int dv, int final_state, int backward);
 int dism_delta_forward(const void *q, const void *k, const void *v, const void *g, const void *beta, int gates_bf16,
                        const float *initial_state, const int32_t *cu_seqlens, int sequences, int n, int key_heads, int heads,

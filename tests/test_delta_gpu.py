@@ -159,6 +159,71 @@ def test_rows_outside_the_documents_are_zeros(flash):
         assert not grad[:, :10].count_nonzero() and not grad[:, 140:].count_nonzero() and torch.isfinite(grad).all()
 
 
+@pytest.mark.parametrize('starts,n', [([1500, 1800, 3700], 4000), ([3990, 4000], 4100), ([0, 30], 4100)])
+def test_rows_outside_the_documents_of_a_long_pack(flash, starts, n):
+    """Long enough for chains cut into segments; the documents begin late or end early."""
+    x = [t.cuda().requires_grad_() for t in reference.operands(5, 1, n, 1, 1, 64, 64)]
+    out = flash.gated_delta_rule(*x, cu_seqlens=torch.tensor(starts, dtype=torch.int32, device='cuda'))
+    dout = torch.randn_like(out)
+    grads = torch.autograd.grad(out, x, dout)
+    assert not out[:, :starts[0]].count_nonzero() and not out[:, starts[-1]:].count_nonzero()
+    part = slice(starts[0], starts[-1])
+    inner = [t.detach()[:, part].contiguous().requires_grad_() for t in x]
+    want = flash.gated_delta_rule(*inner, cu_seqlens=torch.tensor(starts, dtype=torch.int32, device='cuda') - starts[0])
+    near(out[:, part], want.double(), 2 * OUT, 2)
+    for got, expected in zip(grads, torch.autograd.grad(want, inner, dout[:, part].contiguous())):
+        assert not got[:, :starts[0]].count_nonzero() and not got[:, starts[-1]:].count_nonzero()
+        near(got[:, part], expected.double(), 2 * GRAD, 2)
+
+
+def test_mixed_gate_types_partial_gradients_and_second_order(flash):
+    x = reference.operands(13, 1, 100, 1, 2, 64, 64, torch.float32, device='cuda')
+    x[4] = x[4].bfloat16()
+    leaves = [t.clone().requires_grad_() for t in x]
+    out = flash.gated_delta_rule(*leaves)
+    dout = torch.randn_like(out)
+    every = torch.autograd.grad(out, leaves, dout)
+    assert [t.dtype for t in every] == [t.dtype for t in x]
+    only = x[1].clone().requires_grad_()
+    again = flash.gated_delta_rule(x[0], only, *x[2:])
+    assert torch.equal(again, out) and torch.equal(torch.autograd.grad(again, only, dout)[0], every[1])
+    # a key shared by the batch: its gradient is the sum
+    shared = x[1].clone().requires_grad_()
+    two = flash.gated_delta_rule(*[t.expand(2, *t.shape[1:]) if t is not x[1] else shared.expand(2, *t.shape[1:]) for t in x])
+    grad, = torch.autograd.grad(two, shared, dout.expand(2, *dout.shape[1:]))
+    near(grad, 2 * every[1].double(), GRAD, 2)
+    grad, = torch.autograd.grad(flash.gated_delta_rule(x[0], only, *x[2:]).float().sum(), only, create_graph=True)
+    with pytest.raises(RuntimeError, match='not differentiable'):
+        grad.sum().backward()
+
+
+def test_first_call_inside_a_capture(flash):
+    """A shape whose kernels have not run yet is captured at once."""
+    x = [t.requires_grad_() for t in reference.operands(14, 1, 70, 2, 2, 64, 128, device='cuda')]
+    dout = torch.randn_like(x[2])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = flash.gated_delta_rule(*x)
+        grads = torch.autograd.grad(out, x, dout)
+    graph.replay()
+    torch.cuda.synchronize()
+    want = flash.gated_delta_rule(*x)
+    assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(want, x, dout)))
+
+
+def test_a_step_counts_as_a_change_of_the_state(flash):
+    x = reference.operands(15, 2, 1, 1, 1, 32, 32, device='cuda')
+    state = torch.zeros(2, 1, 32, 32, device='cuda')
+    before = state._version
+    flash.gated_delta_step(*[t[:, 0] for t in x], state)
+    assert state._version > before
+    with torch.inference_mode():
+        held = torch.zeros(2, 1, 32, 32, device='cuda')
+        flash.gated_delta_step(*[t[:, 0] for t in x], held)
+    assert torch.equal(held, state)
+
+
 def test_host_and_device_starts_and_layout_agree(flash):
     x = [t.cuda() for t in reference.operands(6, 1, 768, 1, 1, 32, 32)]
     starts = torch.tensor([0, 256, 768], dtype=torch.int32)
