@@ -749,7 +749,10 @@ cudaError_t launch(const CUtensorMap (&x_map)[2], const CUtensorMap (&code_map)[
 }  // namespace
 
 bool encode_rows(CUtensorMap* map, const void* data, uint64_t rows, uint64_t columns, uint64_t row_stride, int box_rows) {
-    return make_map(map, data, rows, columns, row_stride, box_rows);
+    if (make_map(map, data, rows, columns, row_stride, box_rows)) return true;
+    // A thread that has made no runtime call yet (autograd's, at its first backward) has no context for the driver's encoder.
+    int device = 0;
+    return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && make_map(map, data, rows, columns, row_stride, box_rows);
 }
 
 bool labels_tcgen05_covers(const void* x, const void* codebook, int batch, int n, int heads, int d, int vocab) {
