@@ -5,6 +5,15 @@
 // X = T Y, U = b X, O = scale e^G Q S0 + P U, S1 = e^{G_63} S0 + K^T (e^{G_63 - G} U).  Warps share K, Q, T and P of the
 // chunk in shared memory, double-buffered with cp.async; nothing else passes between them.
 //
+// Why a warp per 16 columns: the chain of products has to be short, and with the accumulators of one product as the left operand of the
+// next nothing goes through memory between them.  The same chain on tcgen05 (a thread per column, three round trips through tensor
+// memory a chunk) was built in full and took 2.8 to 3.1 us a chunk, where this chain (then with single operands) took 2.66 for a CTA alone on its SM and 4.7
+// for two.  In us, that one against this: 16 x 2048, 10 heads of 128: 228 / 232; 4 x 8192, 16 heads of 128: 402 / 340; 2 x 8192, 16 heads of
+// 64, uncut: 279 / 209; prompt of 16384, 16 heads of 128, uncut: 850 / 762; 500, 4 heads: 38 to 45 / 27.
+// What bounds it: with four warps a CTA and two CTAs an SM, latency of dependent instructions (one or two warps to a scheduler; the main
+// stall is the fixed latency of an instruction, with one CTA an SM the tensor pipe is 47 % busy).  16 x 2048 positions, 10 heads of 128
+// (320 CTAs for 296 places): 250 us; as segments 2 x 8192, 16 heads of 64: 62 + 66 us.
+//
 // What is rounded: products take bf16, so every operand that is not one already is rounded, once, or kept as a pair (value and
 // remainder, 16 bits) for a second product.  Y and what is added to the state are pairs always: these roundings would reach every
 // later position (with slow decays each alone costs the gradients 2e-3 of their norm, as much as their own rounding to bf16).
@@ -351,7 +360,7 @@ cudaError_t by_width(const DeltaShape& shape, const __nv_bfloat16* q, const __nv
 // A segment costs two CTA walks forward (one of them for B and M, without outputs) and two backward, so cutting pays when the walks
 // get at least four times shorter; with segments of equal length for two CTAs per SM (what the chains' registers and shared memory
 // allow), but no shorter than eight chunks, below which putting the starts together costs what it saves.  Measured, forward and
-// backward chain, uncut / for one / for two CTAs per SM (us): 2 x 8192, 16 heads of 64: 426 / 281 / 211; prompt of 16384, 16 heads of
+// backward chain with single operands, uncut / for one / for two CTAs per SM (us): 2 x 8192, 16 heads of 64: 426 / 281 / 211; prompt of 16384, 16 heads of
 // 128: 761 / 523 / 439; pack of 7019, 8 heads: 166 / 152 / 120.  4 x 2048, 10 heads of 128 (32 chunks to 9): 204 / - / 212.
 int delta_segment_length(const DeltaLayout& layout, int heads, int d, int dv) {
     if (d < 64 || dv < 64) return 0;

@@ -2,6 +2,8 @@
 //     u = b (v - a S^T k),   S <- a S + k u^T,   o = scale S^T q = scale (a S_old^T q + (k.q) u).
 // Both products with the old state come out of one reading of it, so the state is read once and written once and everything
 // is in 32 bits.  A CTA takes 32 columns of one head's state (columns do not interact), held in registers in between.
+// Bound by memory latency (27 % of an SM's warps resident; 72 registers a thread instead of 96 changed nothing): a batch of 96 rows, some
+// padding, 16 heads of 128 x 128 moves 175 MB in 35.8 us, 4.9 TB/s (0.76 of the measured copy rate); one row of 10 heads 6 us.
 #include "delta_common.cuh"
 
 namespace dism {

@@ -7,6 +7,10 @@
 // of it is stored, the backward of a call is the same call on the gradient without a residual, and neither the grid nor the
 // vector width changes it.  Seed and offset are read from device memory when the kernel runs, so a captured graph draws new
 // masks after the program has advanced the offset.
+//
+// 42 million bf16 elements, forward with a residual and backward: 98 us for both, 0.66 of the measured copy rate.  Neither side is
+// saturated: 61 and 65 % of the issue slots, DRAM at 51 and 35 %; stalls are loads first, then the arithmetic pipes.  A grid that fills
+// the device once and loads a block ahead was slower (65 + 52 us against 57.6 + 45.5 between events).
 #include <cuda_fp16.h>
 
 #include "dism_common.cuh"

@@ -170,7 +170,8 @@ int dism_longest_match(const int32_t *streams, int batch, int n, int32_t *end, i
  * cu_seqlens device int32 [sequences+1]; document i is [cu[i], cu[i+1]), any length, empty ones included.  The library cannot
  * read the table on the host: entries are clamped to [0, n], so no table reaches outside the tensors, but the results are
  * defined only for ascending ones; rows before the first and behind the last document come out as zeros.  initial_state NULL: zeros; final_state NULL: not wanted.
- * With a final state the chain of chunks carries its operands as pairs of bf16 (16 bits), without one as single bf16.
+ * The chain of chunks takes V - e^G K S and what it adds to the state as pairs of bf16 (16 bits); with a final state the state and the
+ * chunk's inverse too, without one those are single bf16.
  * `saved`: dism_delta_saved bytes, 256-byte aligned; dead after the call unless `backward` is set: then dism_delta_backward
  * of the same call takes it (a size computed with final_state serves both).  The sizes are those of the current device. */
 size_t dism_delta_saved(int packed, int sequences, int n, int heads, int d, int dv, int final_state, int backward);

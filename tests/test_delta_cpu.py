@@ -112,7 +112,7 @@ def test_document_starts_are_validated_on_the_host(flash):
 
 
 def test_philox_blocks():
-    """The generator of the tests against the published known answers of Philox4x32-10 (Random123's kat_vectors): all zeros, all ones."""
+    """The generator of the tests against the published known answers of Philox4x32-10: all zeros, all ones."""
     import numpy as np
     import delta_reference as reference
     first = reference.philox(8, 0, 0, 0).astype(np.uint32)
