@@ -66,16 +66,30 @@ class _GatedDelta(torch.autograd.Function):
 
 
 _starts = {}
+_captured = {}  # graphs hold the addresses of these
+
+
+def _capturing(device):
+    return device.type == 'cuda' and torch.cuda.is_current_stream_capturing()
 
 
 def _host_starts(starts, device):
-    """Uploads document starts once per distinct pack and device."""
+    """Document starts on the device, uploaded once for as long as the pack is among the last 32 or a captured graph reads it."""
     key = (tuple(starts), str(device))
-    cached = _starts.get(key)
+    cached = _captured.get(key)
+    if cached is None:
+        cached = _starts.get(key)
+    if _capturing(device):
+        if cached is None:
+            raise RuntimeError('document starts cannot be uploaded inside a capture: make the call once before it, or pass cu_seqlens on the device')
+        _captured[key] = cached
+        return cached
     if cached is None:
         if len(_starts) >= 32:
-            _starts.pop(next(iter(_starts)))
+            _starts.pop(next(iter(_starts)), None)
         cached = _starts[key] = torch.tensor(starts, dtype=torch.int32).to(device)
+    if device.type == 'cuda':
+        cached.record_stream(torch.cuda.current_stream(device))  # dropped, its memory waits for this call's kernels
     return cached
 
 
@@ -109,7 +123,8 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, output
     H is a multiple of HK (value head h reads key head h // (H // HK)), D and DV in {32,64,128}, N any length.  Keys are meant to
     have length one at most; the caller normalises.  scale defaults to D ** -0.5.  g = -inf clears the state.  A pack is one
     batch row with either `layout` (a VarlenLayout) or `cu_seqlens`, int32 [documents+1]; documents may have any length, zero
-    included.  On the CPU cu_seqlens is validated; on the GPU it is read by the kernels only (so a captured graph can follow new
+    included.  On the CPU cu_seqlens is validated (and like a layout uploaded once, which has to happen before a
+    capture); on the GPU it is read by the kernels only (so a captured graph can follow new
     lengths), must ascend, and rows outside [cu_seqlens[0], cu_seqlens[-1]) come out as zeros.  initial_state is FP32
     [sequences,H,D,DV].  All operands and the initial state are differentiable; gates receive gradients in their own type, with
     the relative accuracy of the bf16 operands.  Keeping the states for a backward takes 2 D DV / 64 + 2 DV + 184 bytes per position

@@ -111,6 +111,20 @@ def test_document_starts_are_validated_on_the_host(flash):
     assert delta._documents(v, torch.tensor([0, 3, 3, 8], dtype=torch.int32), None).tolist() == [0, 3, 3, 8]
 
 
+def test_host_starts_that_a_capture_uses_are_never_dropped(flash, monkeypatch):
+    from flash_dism import delta
+    upload = lambda starts: delta._host_starts(starts, torch.device('cpu'))
+    first = upload([0, 11])
+    monkeypatch.setattr(delta, '_capturing', lambda device: True, raising=False)
+    assert upload([0, 11]) is first
+    with pytest.raises(RuntimeError, match='inside a capture'):
+        upload([0, 12])
+    monkeypatch.setattr(delta, '_capturing', lambda device: False, raising=False)
+    others = [upload([0, i]) for i in range(100, 200)]
+    assert upload([0, 11]) is first and upload([0, 199]) is others[-1]
+    assert len(delta._starts) <= 32
+
+
 def test_philox_blocks():
     """The generator of the tests against the published known answers of Philox4x32-10: all zeros, all ones."""
     import numpy as np

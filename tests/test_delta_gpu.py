@@ -292,6 +292,36 @@ def test_another_stream_and_graph_replay(flash):
         assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+def test_a_captured_pack_outlives_others_and_a_first_upload_inside_a_capture_is_refused(flash):
+    x = [t.cuda() for t in reference.operands(12, 1, 200, 2, 2, 64, 64)]
+    starts = torch.tensor([0, 71, 200], dtype=torch.int32)
+    want = flash.gated_delta_rule(*x, cu_seqlens=starts)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = flash.gated_delta_rule(*x, cu_seqlens=starts)
+        with pytest.raises(RuntimeError, match='inside a capture'):
+            flash.gated_delta_rule(*x, cu_seqlens=torch.tensor([0, 72, 200], dtype=torch.int32))
+    for i in range(80, 120):
+        flash.gated_delta_rule(*x, cu_seqlens=torch.tensor([0, i, 200], dtype=torch.int32))
+    taken = [torch.full((64,), 5, dtype=torch.int32, device='cuda') for _ in range(200)]
+    got.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and len(taken) == 200
+
+
+@pytest.mark.parametrize('n,d', [(200, 64), (2100, 64), (130, 32)])
+def test_a_graph_can_be_walked_twice(flash, n, d):
+    """The kept states are read only: a second backward pass of one forward gives the same gradients, chains cut or not."""
+    x = [t.cuda().requires_grad_() for t in reference.operands(13, 1, n, 1, 2, d, 64)]
+    out, final = flash.gated_delta_rule(*x, output_final_state=True)
+    dout, dfinal = torch.randn_like(out), torch.randn_like(final)
+    first = torch.autograd.grad((out, final), x, (dout, dfinal), retain_graph=True)
+    second = torch.autograd.grad((out, final), x, (dout, dfinal))
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+
+
 def test_two_calls_at_once(flash):
     """Two streams, each with its own call in flight many times over, do not disturb one another."""
     sets = [[t.cuda().requires_grad_() for t in reference.operands(s, 1, 500, 2, 2, 64, 64)] for s in (1, 2)]
