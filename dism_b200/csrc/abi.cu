@@ -336,23 +336,31 @@ size_t lay_out_delta(dism::DeltaShape& shape, bool exact, bool backward, char* b
     if (exact) shape.segments.m_rest = reinterpret_cast<bf*>(take(segments * shape.d * shape.d * 2));
     shape.segments.ends = reinterpret_cast<float*>(take(segments * shape.d * shape.dv * 4));
     if (exact) parts.t_rest = reinterpret_cast<bf*>(take(places * dism::MATRIX * 2));
+    if (shape.shares.length) {
+        shape.shares.states = reinterpret_cast<float*>(take(size_t(shape.shares.places) * shape.d * dism::CHUNK * 4));
+        shape.shares.flags = reinterpret_cast<unsigned*>(take(shape.shares.flag_bytes()));
+    }
     if (saved) *saved = parts;
     return at;
 }
-size_t delta_scratch(const dism::DeltaShape& shape, char* base, dism::DeltaGradients* x) {
+size_t delta_scratch(dism::DeltaShape& shape, char* base, dism::DeltaGradients* x) {
     const size_t places = size_t(shape.layout.slots()) * shape.heads;
     const size_t segments = shape.segments.length ? size_t(shape.segments.count(shape.layout)) * shape.heads : 0;
     const size_t states = round_up(places * shape.d * shape.dv * 2), parts = round_up(places * dism::CHUNK * (shape.dv / 16) * 4);
+    const size_t ends = round_up(segments * shape.d * shape.dv * 4), shares = shape.shares.length ? round_up(size_t(shape.shares.places) * shape.d * dism::CHUNK * 4) : 0;
     if (x) {
         x->dstates = reinterpret_cast<__nv_bfloat16*>(base);
         x->dbeta_parts = reinterpret_cast<float*>(base + states);
         x->ends = reinterpret_cast<float*>(base + states + parts);
+        shape.shares.states = reinterpret_cast<float*>(base + states + parts + ends);
+        shape.shares.flags = reinterpret_cast<unsigned*>(base + states + parts + ends + shares);
     }
-    return states + parts + round_up(segments * shape.d * shape.dv * 4);
+    return states + parts + ends + shares + (shares ? round_up(shape.shares.flag_bytes()) : 0);
 }
 dism::DeltaShape delta_shape(const int32_t* cu_seqlens, int sequences, int n, int key_heads, int heads, int d, int dv, int gates_bf16, float scale) {
     const dism::DeltaLayout layout{cu_seqlens, sequences, n};
-    return dism::DeltaShape{layout, dism::DeltaSegments{dism::delta_segment_length(layout, heads, d, dv), nullptr, nullptr, nullptr}, key_heads, heads, d, dv, gates_bf16 != 0, scale};
+    return dism::DeltaShape{layout, dism::DeltaSegments{dism::delta_segment_length(layout, heads, d, dv), nullptr, nullptr, nullptr},
+                            dism::delta_shares(layout, heads, d, dv), key_heads, heads, d, dv, gates_bf16 != 0, scale};
 }
 }  // namespace
 

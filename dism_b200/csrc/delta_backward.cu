@@ -3,7 +3,7 @@
 //     dS0 = e^{G_63} dS1 + (scale e^G Q)^T dO - (e^G K)^T dY.
 // delta_reverse_kernel walks the chunks from the last to the first with dS, transposed, in its accumulators (a warp owns 16
 // columns, as in the forward chain), writes dV, keeps every dS1 and the part of db that needs dU.
-// As the forward chain it is bound by latency: 236 us at 16 x 2048 positions, 10 heads of 128; segments of 2 x 8192, 16 heads of 64: 39 + 64.
+// As the forward chain it is bound by latency: 166 us at 16 x 2048 positions, 10 heads of 128 (in shares); segments of 2 x 8192, 16 heads of 64: 39 + 64.
 // delta_gradient_kernel then takes all chunks at once (here for D or DV of 32; delta_gradient.cu has the others).  With Z1 = dO X^T and Z2 = dY X^T,
 //     dP~ = scale E b_s Z1 (s <= t),   dL~ = -E b_s Z2 (s < t),
 //     dQ = scale e^G dO S0^T + dP~ K,
@@ -26,265 +26,289 @@ struct ReverseStage {
     static constexpr int X = 2 * BYTES, TOTAL = X + CHUNK * VALUE_PITCH;  // one X for both stages: its columns belong to a warp each
 };
 
+__device__ int delta_reverse_fault;
+
 // LOCAL: the first launch over segments: from a zero gradient behind the segment to the one before it, no outputs.
-template <int D, int WARPS, bool LOCAL>
+// SHARES: a part of an uncut chain (see DeltaShares), its chunks counted from the end.
+template <int D, int WARPS, bool LOCAL, bool SHARES>
 __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape shape, const __nv_bfloat16* __restrict__ q,
-                                                                   const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ dout,
-                                                                   const float* __restrict__ dfinal, DeltaSaved saved,
-                                                                   __nv_bfloat16* __restrict__ dstates, float* __restrict__ dbeta_parts,
-                                                                   __nv_bfloat16* __restrict__ dv_out, float* __restrict__ dinitial, float* __restrict__ ends) {
+                                                                      const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ dout,
+                                                                      const float* __restrict__ dfinal, DeltaSaved saved,
+                                                                      __nv_bfloat16* __restrict__ dstates, float* __restrict__ dbeta_parts,
+                                                                      __nv_bfloat16* __restrict__ dv_out, float* __restrict__ dinitial, float* __restrict__ ends) {
     using Stage = ReverseStage<D, WARPS>;
     constexpr int THREADS = WARPS * 32, TILES = CHUNK / 8;
     extern __shared__ __align__(128) unsigned char shared[];
     const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
-    const int head = blockIdx.y, dv = shape.dv;
-    const int key_head = head / (shape.heads / shape.key_heads), column = (blockIdx.z * WARPS + warp) * 16;
-    int64_t row, slot;
-    int length, sequence, number;
-    shape.segments.find(shape.layout, blockIdx.x, sequence, number);
-    if (number < 0) return;  // segments before the first document
-    shape.layout.span(sequence, row, length, slot);
-    const unsigned base = smem_address(shared);
-    if (!LOCAL && shape.layout.cu && number == 0) {
-        char* to = reinterpret_cast<char*>(dv_out + int64_t(head) * dv + blockIdx.z * WARPS * 16);
-        const int64_t stride = int64_t(shape.heads) * dv * 2;
-        if (sequence == 0) clear_rows<WARPS * 32>(to, stride, WARPS * 2, 0, row, thread);
-        if (sequence == shape.layout.sequences - 1) clear_rows<WARPS * 32>(to, stride, WARPS * 2, row + length, shape.layout.n, thread);
-    }
-    int chunks = (length + CHUNK - 1) / CHUNK, behind = 0;  // segments behind this one
-    if (shape.segments.length) {
-        const int before = min(number * shape.segments.length, chunks);
-        if (number && before == chunks) return;  // no such segment
-        if (LOCAL && number == 0) return;
-        behind = (chunks - 1 - before) / shape.segments.length;
-        chunks = min(chunks - before, shape.segments.length);
-        slot += before, row += int64_t(before) * CHUNK, length -= before * CHUNK;
-    }
-    const int64_t key_stride = int64_t(shape.key_heads) * D * 2, value_stride = int64_t(shape.heads) * dv * 2;
-    auto load = [&](int c) {
-        const unsigned stage = base + (c & 1) * Stage::BYTES;
-        const int count = min(CHUNK, length - c * CHUNK);
-        const int64_t at = row + int64_t(c) * CHUNK, place = (slot + c) * shape.heads + head;
-        const int64_t key = (at * shape.key_heads + key_head) * D * 2;
-        load_tile<2 * D, THREADS>(stage + Stage::K, reinterpret_cast<const char*>(k) + key, key_stride, count, thread);
-        load_tile<32 * WARPS, THREADS>(stage + Stage::DOUT,
-                                       reinterpret_cast<const char*>(dout) + ((at * shape.heads + head) * dv + blockIdx.z * WARPS * 16) * 2,
-                                       value_stride, count, thread);
-        load_block<3 * CHUNK * 4, THREADS>(stage + Stage::ROWS, reinterpret_cast<const char*>(saved.rows + place * ROW_VALUES), thread);
-        load_block<2 * MATRIX, THREADS>(stage + Stage::P, reinterpret_cast<const char*>(saved.p + place * MATRIX), thread);
-        load_block<2 * MATRIX, THREADS>(stage + Stage::T, reinterpret_cast<const char*>(saved.t + place * MATRIX), thread);
-        load_tile<2 * D, THREADS>(stage + Stage::Q, reinterpret_cast<const char*>(q) + key, key_stride, count, thread);
-        cp_async_commit();
-    };
-
-    float ds[D / 8][4];
-    const int64_t state_at = (int64_t(sequence) * shape.heads + head) * D * dv + column + (lane >> 2);
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            // the gradient behind the sequence; a segment that is not the last starts from zero in the first launch
-            ds[n][e] = dfinal && (!LOCAL || behind == 0) ? __ldg(dfinal + state_at + int64_t(8 * n + 2 * (lane & 3) + (e & 1)) * dv + (e >> 1) * 8) : 0.f;
-    // the gradient behind an earlier segment: dS <- M^T dS + B over the segments behind it.  The last one's B already has dfinal.
-    if (!LOCAL)
-        for (int later = behind; later > 0; --later) {
-            const int64_t place = (int64_t(blockIdx.x) + later) * shape.heads + head;
-            const float4* end = reinterpret_cast<const float4*>(ends + place * D * dv) + column / 16 * (D / 8) * 32 + lane;
-            float x[D / 8][4];
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float4*>(x[n]) = __ldg(end + n * 32);
-            if (later < behind) {
-                load_block<2 * D * D, THREADS>(base, reinterpret_cast<const char*>(shape.segments.m + place * D * D), thread);
-                cp_async_commit();
-                cp_async_wait<0>();
-                __syncthreads();
-#pragma unroll
-                for (int kb = 0; kb < D / 16; ++kb) {
-                    unsigned a[4];
-                    to_operand(a, ds[2 * kb], ds[2 * kb + 1]);
-#pragma unroll
-                    for (int np = 0; np < D / 16; ++np) {
-                        unsigned b[4];
-                        ldsm4(b, base + (np * 2 * (D / 8) + kb * 2) * 128 + cols_first_blocked(lane, D / 8));
-                        mma16816(x[2 * np], a, b[0], b[1]);
-                        mma16816(x[2 * np + 1], a, b[2], b[3]);
-                    }
-                }
-                __syncthreads();
-            }
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) ds[n][e] = x[n][e];
+    ShareWalk<D * 16 * WARPS> share;
+    if (SHARES && !share.draw(shape, WARPS * 16)) return;
+    bool more = false;
+    do {
+        const DeltaPart part = SHARES ? share.part(shape, &delta_reverse_fault, 12) : DeltaPart{blockIdx.x, blockIdx.y, blockIdx.z, 0, 0, nullptr, nullptr};
+        const int head = part.head, dv = shape.dv;
+        const int key_head = head / (shape.heads / shape.key_heads), column = (part.block * WARPS + warp) * 16;
+        int64_t row, slot;
+        int length, sequence, number;
+        if (SHARES) sequence = part.segment, number = 0;
+        else shape.segments.find(shape.layout, part.segment, sequence, number);
+        if (number < 0) return;  // segments before the first document
+        shape.layout.span(sequence, row, length, slot);
+        const unsigned base = smem_address(shared);
+        if (!LOCAL && !SHARES && shape.layout.cu && number == 0) {
+            char* to = reinterpret_cast<char*>(dv_out + int64_t(head) * dv + part.block * WARPS * 16);
+            const int64_t stride = int64_t(shape.heads) * dv * 2;
+            if (sequence == 0) clear_rows<WARPS * 32>(to, stride, WARPS * 2, 0, row, thread);
+            if (sequence == shape.layout.sequences - 1) clear_rows<WARPS * 32>(to, stride, WARPS * 2, row + length, shape.layout.n, thread);
         }
-    if (chunks > 0) load(chunks - 1);
-    for (int c = chunks - 1; c >= 0; --c) {
-        cp_async_wait<0>();
-        __syncthreads();  // chunk c is in, and every warp has left chunk c + 1
-        if (!LOCAL) {  // X of this chunk, transposed: the warp's own rows, two kilobytes, needed only after dU
-            const char* from = reinterpret_cast<const char*>(saved.x + ((slot + c) * shape.heads + head) * CHUNK * dv + column * CHUNK);
-#pragma unroll
-            for (int i = lane * 16; i < 2048; i += 512)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + Stage::X + warp * 2048 + i), "l"(from + i));
-            cp_async_commit();
+        int chunks = (length + CHUNK - 1) / CHUNK, behind = 0;  // segments behind this one
+        if (SHARES) {
+            const int before = chunks - part.end;
+            chunks = part.end - part.begin;
+            slot += before, row += int64_t(before) * CHUNK, length -= before * CHUNK;
+        } else if (shape.segments.length) {
+            const int before = min(number * shape.segments.length, chunks);
+            if (number && before == chunks) return;  // no such segment
+            if (LOCAL && number == 0) return;
+            behind = (chunks - 1 - before) / shape.segments.length;
+            chunks = min(chunks - before, shape.segments.length);
+            slot += before, row += int64_t(before) * CHUNK, length -= before * CHUNK;
         }
-        if (c > 0) load(c - 1);
-        else cp_async_commit();
-        const unsigned stage = base + (c & 1) * Stage::BYTES;
-        const float* rows = reinterpret_cast<const float*>(shared + (c & 1) * Stage::BYTES + Stage::ROWS);
-        const int64_t place = (slot + c) * shape.heads + head;
-
-        float du[TILES][4];
-#pragma unroll
-        for (int n = 0; n < TILES; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) du[n][e] = 0.f;
-        const TileLane keys = tile_cols_first<Stage::PITCH>(stage + Stage::K, lane);
-        unsigned* state_out = reinterpret_cast<unsigned*>(dstates + place * dv * D) + int64_t(column / 8) * (D / 8) * 32 + lane;
-#pragma unroll
-        for (int kb = 0; kb < D / 16; ++kb) {
-            unsigned a[4];
-            to_operand(a, ds[2 * kb], ds[2 * kb + 1]);
-            if (!LOCAL) {
-                unsigned* to = state_out + 2 * kb * 32;
-                to[0] = a[0], to[D / 8 * 32] = a[1], to[32] = a[2], to[D / 8 * 32 + 32] = a[3];
-            }
-#pragma unroll
-            for (int np = 0; np < TILES / 2; ++np) {
-                unsigned b[4];
-                ldsm4(b, keys.at(kb * 32) + np * 16 * Stage::PITCH);
-                mma16816(du[2 * np], a, b[0], b[1]);
-                mma16816(du[2 * np + 1], a, b[2], b[3]);
-            }
-        }
-        const unsigned own = tile_cols_first<Stage::VALUE_PITCH>(0, lane).at(warp * 32);
-        unsigned grad[TILES / 2][4];  // dO, transposed, as a left operand
-#pragma unroll
-        for (int np = 0; np < TILES / 2; ++np) {
-            ldsm4_trans(grad[np], stage + Stage::DOUT + own + np * 16 * Stage::VALUE_PITCH);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float2 tail = *reinterpret_cast<const float2*>(rows + 2 * CHUNK + 16 * np + 8 * h + 2 * (lane & 3));
-                float(&tile)[4] = du[2 * np + h];
-                tile[0] *= tail.x, tile[1] *= tail.y, tile[2] *= tail.x, tile[3] *= tail.y;
-            }
-        }
-        const unsigned inside = stage + Stage::P + rows_first_tile(lane), inverse = inside + Stage::T - Stage::P;
-#pragma unroll
-        for (int np = 0; np < TILES / 2; ++np)
-#pragma unroll
-            for (int kb = np; kb < TILES / 2; ++kb) {
-                unsigned b[4];
-                ldsm4_trans(b, inside + tile_at(kb, np));
-                mma16816(du[2 * np], grad[kb], b[0], b[1]);
-                mma16816(du[2 * np + 1], grad[kb], b[2], b[3]);
-            }
-        // the part of db that needs dU: this warp's 16 columns of dU.X
-        float* part = dbeta_parts + (int64_t(column / 16) * shape.layout.slots() * shape.heads + place) * CHUNK;
-        unsigned dx[TILES / 2][4], dx_rest[TILES / 2][4];  // a pair: its rounding would be one more in dV and in all that follows
-        cp_async_wait<1>();  // all but the next chunk
-        __syncwarp();
-#pragma unroll
-        for (int np = 0; np < TILES / 2; ++np) {
-            unsigned xx[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int e = 0; e < 4 && !LOCAL; ++e) xx[e] = *reinterpret_cast<const unsigned*>(shared + Stage::X + warp * 2048 + ((e & 1) * TILES + 2 * np + (e >> 1)) * 128 + lane * 4);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float(&tile)[4] = du[2 * np + h];
-                if (!LOCAL) {
-                    float even = tile[0] * low_half(xx[2 * h]) + tile[2] * low_half(xx[2 * h + 1]);
-                    float odd = tile[1] * high_half(xx[2 * h]) + tile[3] * high_half(xx[2 * h + 1]);
-#pragma unroll
-                    for (int m = 4; m < 32; m <<= 1) even += __shfl_xor_sync(FULL, even, m), odd += __shfl_xor_sync(FULL, odd, m);
-                    if (lane < 4) *reinterpret_cast<float2*>(part + 16 * np + 8 * h + 2 * lane) = make_float2(even, odd);
-                }
-                const float2 b = *reinterpret_cast<const float2*>(rows + CHUNK + 16 * np + 8 * h + 2 * (lane & 3));
-                tile[0] *= b.x, tile[1] *= b.y, tile[2] *= b.x, tile[3] *= b.y;
-            }
-            to_operand(dx[np], du[2 * np], du[2 * np + 1]);
-            to_operand_rest(dx_rest[np], dx[np], du[2 * np], du[2 * np + 1]);
-        }
-        float(&dy)[TILES][4] = du;
-#pragma unroll
-        for (int n = 0; n < TILES; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dy[n][e] = 0.f;
-#pragma unroll
-        for (int np = 0; np < TILES / 2; ++np)
-#pragma unroll
-            for (int kb = np; kb < TILES / 2; ++kb) {
-                unsigned b[4];
-                ldsm4_trans(b, inverse + tile_at(kb, np));
-                mma16816(dy[2 * np], dx[kb], b[0], b[1]);
-                mma16816(dy[2 * np + 1], dx[kb], b[2], b[3]);
-                mma16816(dy[2 * np], dx_rest[kb], b[0], b[1]);
-                mma16816(dy[2 * np + 1], dx_rest[kb], b[2], b[3]);
-            }
-        if (!LOCAL) {
-            // dV leaves through the warp's room of X: rows of 32 bytes, the halves of rows 4-7 of every eight exchanged
-            const unsigned values = base + Stage::X + warp * 2048 + ((lane & 7) + ((lane >> 4) << 3)) * 32 + ((((lane >> 3) ^ (lane >> 2)) & 1) * 16);
-            __syncwarp();
-#pragma unroll
-            for (int np = 0; np < TILES / 2; ++np)
-                stsm4_trans(values + np * 512, pack2(dy[2 * np][0], dy[2 * np][1]), pack2(dy[2 * np][2], dy[2 * np][3]),
-                            pack2(dy[2 * np + 1][0], dy[2 * np + 1][1]), pack2(dy[2 * np + 1][2], dy[2 * np + 1][3]));
-            __syncwarp();
+        const int64_t key_stride = int64_t(shape.key_heads) * D * 2, value_stride = int64_t(shape.heads) * dv * 2;
+        auto load = [&](int c) {
+            const unsigned stage = base + (c & 1) * Stage::BYTES;
             const int count = min(CHUNK, length - c * CHUNK);
-            char* to = reinterpret_cast<char*>(dv_out + ((row + int64_t(c) * CHUNK) * shape.heads + head) * dv + column);
-#pragma unroll
-            for (int i = 0; i < CHUNK * 2 / 32; ++i) {
-                const int t = i * 16 + (lane >> 1);
-                const uint4 piece = *reinterpret_cast<const uint4*>(shared + Stage::X + warp * 2048 + t * 32 + (((lane & 1) ^ ((t >> 2) & 1)) * 16));
-                if (t < count) *reinterpret_cast<uint4*>(to + t * value_stride + (lane & 1) * 16) = piece;
-            }
-            __syncwarp();  // the room is free for the next chunk's X
-        }
-        // scale e^G dO and -e^G dY, the left operands of the state's step
-#pragma unroll
-        for (int np = 0; np < TILES / 2; ++np) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float2 decay = *reinterpret_cast<const float2*>(rows + 16 * np + 8 * h + 2 * (lane & 3));
-                const float sx = shape.scale * decay.x, sy = shape.scale * decay.y;
-                float(&tile)[4] = dy[2 * np + h];
-                tile[0] *= -decay.x, tile[1] *= -decay.y, tile[2] *= -decay.x, tile[3] *= -decay.y;
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    grad[np][2 * h + e] = pack2(low_half(grad[np][2 * h + e]) * sx, high_half(grad[np][2 * h + e]) * sy);
-            }
-            to_operand(dx[np], dy[2 * np], dy[2 * np + 1]);
-        }
-        const float kept = rows[CHUNK - 1];
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ds[n][e] *= kept;
-        const TileLane keys_trans = tile_rows_first<Stage::PITCH>(stage + Stage::K, lane);
-#pragma unroll
-        for (int kb = 0; kb < TILES / 2; ++kb)
-#pragma unroll
-            for (int np = 0; np < D / 16; ++np) {
-                unsigned b[4];
-                ldsm4_trans(b, keys_trans.at(np * 32) + kb * 16 * Stage::PITCH);
-                mma16816(ds[2 * np], dx[kb], b[0], b[1]);
-                mma16816(ds[2 * np + 1], dx[kb], b[2], b[3]);
-                ldsm4_trans(b, keys_trans.at(np * 32) + Stage::Q - Stage::K + kb * 16 * Stage::PITCH);
-                mma16816(ds[2 * np], grad[kb], b[0], b[1]);
-                mma16816(ds[2 * np + 1], grad[kb], b[2], b[3]);
-            }
-    }
-    if (LOCAL) {
-        float4* to = reinterpret_cast<float4*>(ends + (int64_t(blockIdx.x) * shape.heads + head) * D * dv) + column / 16 * (D / 8) * 32 + lane;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) to[n * 32] = *reinterpret_cast<float4*>(ds[n]);
-    } else if (dinitial && number == 0) {
+            const int64_t at = row + int64_t(c) * CHUNK, place = (slot + c) * shape.heads + head;
+            const int64_t key = (at * shape.key_heads + key_head) * D * 2;
+            load_tile<2 * D, THREADS>(stage + Stage::K, reinterpret_cast<const char*>(k) + key, key_stride, count, thread);
+            load_tile<32 * WARPS, THREADS>(stage + Stage::DOUT,
+                                           reinterpret_cast<const char*>(dout) + ((at * shape.heads + head) * dv + part.block * WARPS * 16) * 2,
+                                           value_stride, count, thread);
+            load_block<3 * CHUNK * 4, THREADS>(stage + Stage::ROWS, reinterpret_cast<const char*>(saved.rows + place * ROW_VALUES), thread);
+            load_block<2 * MATRIX, THREADS>(stage + Stage::P, reinterpret_cast<const char*>(saved.p + place * MATRIX), thread);
+            load_block<2 * MATRIX, THREADS>(stage + Stage::T, reinterpret_cast<const char*>(saved.t + place * MATRIX), thread);
+            load_tile<2 * D, THREADS>(stage + Stage::Q, reinterpret_cast<const char*>(q) + key, key_stride, count, thread);
+            cp_async_commit();
+        };
+
+        float ds[D / 8][4];
+        const int64_t state_at = (int64_t(sequence) * shape.heads + head) * D * dv + column + (lane >> 2);
 #pragma unroll
         for (int n = 0; n < D / 8; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                dinitial[state_at + int64_t(8 * n + 2 * (lane & 3) + (e & 1)) * dv + (e >> 1) * 8] = ds[n][e];
-    }
+                // the gradient behind the sequence; a segment that is not the last starts from zero in the first launch
+                if (!SHARES || !part.from) ds[n][e] = dfinal && (!LOCAL || behind == 0) ? __ldg(dfinal + state_at + int64_t(8 * n + 2 * (lane & 3) + (e & 1)) * dv + (e >> 1) * 8) : 0.f;
+        if (SHARES && part.from) {
+            const float4* from = reinterpret_cast<const float4*>(part.from) + warp * (D / 8) * 32 + lane;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float4*>(ds[n]) = __ldcg(from + n * 32);
+        }
+        // the gradient behind an earlier segment: dS <- M^T dS + B over the segments behind it.  The last one's B already has dfinal.
+        if (!LOCAL && !SHARES)
+            for (int later = behind; later > 0; --later) {
+                const int64_t place = (int64_t(part.segment) + later) * shape.heads + head;
+                const float4* end = reinterpret_cast<const float4*>(ends + place * D * dv) + column / 16 * (D / 8) * 32 + lane;
+                float x[D / 8][4];
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float4*>(x[n]) = __ldg(end + n * 32);
+                if (later < behind) {
+                    load_block<2 * D * D, THREADS>(base, reinterpret_cast<const char*>(shape.segments.m + place * D * D), thread);
+                    cp_async_commit();
+                    cp_async_wait<0>();
+                    __syncthreads();
+#pragma unroll
+                    for (int kb = 0; kb < D / 16; ++kb) {
+                        unsigned a[4];
+                        to_operand(a, ds[2 * kb], ds[2 * kb + 1]);
+#pragma unroll
+                        for (int np = 0; np < D / 16; ++np) {
+                            unsigned b[4];
+                            ldsm4(b, base + (np * 2 * (D / 8) + kb * 2) * 128 + cols_first_blocked(lane, D / 8));
+                            mma16816(x[2 * np], a, b[0], b[1]);
+                            mma16816(x[2 * np + 1], a, b[2], b[3]);
+                        }
+                    }
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) ds[n][e] = x[n][e];
+            }
+        if (chunks > 0) load(chunks - 1);
+        for (int c = chunks - 1; c >= 0; --c) {
+            cp_async_wait<0>();
+            __syncthreads();  // chunk c is in, and every warp has left chunk c + 1
+            if (!LOCAL) {  // X of this chunk, transposed: the warp's own rows, two kilobytes, needed only after dU
+                const char* from = reinterpret_cast<const char*>(saved.x + ((slot + c) * shape.heads + head) * CHUNK * dv + column * CHUNK);
+#pragma unroll
+                for (int i = lane * 16; i < 2048; i += 512)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + Stage::X + warp * 2048 + i), "l"(from + i));
+                cp_async_commit();
+            }
+            if (c > 0) load(c - 1);
+            else cp_async_commit();
+            const unsigned stage = base + (c & 1) * Stage::BYTES;
+            const float* rows = reinterpret_cast<const float*>(shared + (c & 1) * Stage::BYTES + Stage::ROWS);
+            const int64_t place = (slot + c) * shape.heads + head;
+
+            float du[TILES][4];
+#pragma unroll
+            for (int n = 0; n < TILES; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) du[n][e] = 0.f;
+            const TileLane keys = tile_cols_first<Stage::PITCH>(stage + Stage::K, lane);
+            unsigned* state_out = reinterpret_cast<unsigned*>(dstates + place * dv * D) + int64_t(column / 8) * (D / 8) * 32 + lane;
+#pragma unroll
+            for (int kb = 0; kb < D / 16; ++kb) {
+                unsigned a[4];
+                to_operand(a, ds[2 * kb], ds[2 * kb + 1]);
+                if (!LOCAL) {
+                    unsigned* to = state_out + 2 * kb * 32;
+                    to[0] = a[0], to[D / 8 * 32] = a[1], to[32] = a[2], to[D / 8 * 32 + 32] = a[3];
+                }
+#pragma unroll
+                for (int np = 0; np < TILES / 2; ++np) {
+                    unsigned b[4];
+                    ldsm4(b, keys.at(kb * 32) + np * 16 * Stage::PITCH);
+                    mma16816(du[2 * np], a, b[0], b[1]);
+                    mma16816(du[2 * np + 1], a, b[2], b[3]);
+                }
+            }
+            const unsigned own = tile_cols_first<Stage::VALUE_PITCH>(0, lane).at(warp * 32);
+            unsigned grad[TILES / 2][4];  // dO, transposed, as a left operand
+#pragma unroll
+            for (int np = 0; np < TILES / 2; ++np) {
+                ldsm4_trans(grad[np], stage + Stage::DOUT + own + np * 16 * Stage::VALUE_PITCH);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float2 tail = *reinterpret_cast<const float2*>(rows + 2 * CHUNK + 16 * np + 8 * h + 2 * (lane & 3));
+                    float(&tile)[4] = du[2 * np + h];
+                    tile[0] *= tail.x, tile[1] *= tail.y, tile[2] *= tail.x, tile[3] *= tail.y;
+                }
+            }
+            const unsigned inside = stage + Stage::P + rows_first_tile(lane), inverse = inside + Stage::T - Stage::P;
+#pragma unroll
+            for (int np = 0; np < TILES / 2; ++np)
+#pragma unroll
+                for (int kb = np; kb < TILES / 2; ++kb) {
+                    unsigned b[4];
+                    ldsm4_trans(b, inside + tile_at(kb, np));
+                    mma16816(du[2 * np], grad[kb], b[0], b[1]);
+                    mma16816(du[2 * np + 1], grad[kb], b[2], b[3]);
+                }
+            // the part of db that needs dU: this warp's 16 columns of dU.X
+            float* part = dbeta_parts + (int64_t(column / 16) * shape.layout.slots() * shape.heads + place) * CHUNK;
+            unsigned dx[TILES / 2][4], dx_rest[TILES / 2][4];  // a pair: its rounding would be one more in dV and in all that follows
+            cp_async_wait<1>();  // all but the next chunk
+            __syncwarp();
+#pragma unroll
+            for (int np = 0; np < TILES / 2; ++np) {
+                unsigned xx[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 4 && !LOCAL; ++e) xx[e] = *reinterpret_cast<const unsigned*>(shared + Stage::X + warp * 2048 + ((e & 1) * TILES + 2 * np + (e >> 1)) * 128 + lane * 4);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float(&tile)[4] = du[2 * np + h];
+                    if (!LOCAL) {
+                        float even = tile[0] * low_half(xx[2 * h]) + tile[2] * low_half(xx[2 * h + 1]);
+                        float odd = tile[1] * high_half(xx[2 * h]) + tile[3] * high_half(xx[2 * h + 1]);
+#pragma unroll
+                        for (int m = 4; m < 32; m <<= 1) even += __shfl_xor_sync(FULL, even, m), odd += __shfl_xor_sync(FULL, odd, m);
+                        if (lane < 4) *reinterpret_cast<float2*>(part + 16 * np + 8 * h + 2 * lane) = make_float2(even, odd);
+                    }
+                    const float2 b = *reinterpret_cast<const float2*>(rows + CHUNK + 16 * np + 8 * h + 2 * (lane & 3));
+                    tile[0] *= b.x, tile[1] *= b.y, tile[2] *= b.x, tile[3] *= b.y;
+                }
+                to_operand(dx[np], du[2 * np], du[2 * np + 1]);
+                to_operand_rest(dx_rest[np], dx[np], du[2 * np], du[2 * np + 1]);
+            }
+            float(&dy)[TILES][4] = du;
+#pragma unroll
+            for (int n = 0; n < TILES; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dy[n][e] = 0.f;
+#pragma unroll
+            for (int np = 0; np < TILES / 2; ++np)
+#pragma unroll
+                for (int kb = np; kb < TILES / 2; ++kb) {
+                    unsigned b[4];
+                    ldsm4_trans(b, inverse + tile_at(kb, np));
+                    mma16816(dy[2 * np], dx[kb], b[0], b[1]);
+                    mma16816(dy[2 * np + 1], dx[kb], b[2], b[3]);
+                    mma16816(dy[2 * np], dx_rest[kb], b[0], b[1]);
+                    mma16816(dy[2 * np + 1], dx_rest[kb], b[2], b[3]);
+                }
+            if (!LOCAL) {
+                // dV leaves through the warp's room of X: rows of 32 bytes, the halves of rows 4-7 of every eight exchanged
+                const unsigned values = base + Stage::X + warp * 2048 + ((lane & 7) + ((lane >> 4) << 3)) * 32 + ((((lane >> 3) ^ (lane >> 2)) & 1) * 16);
+                __syncwarp();
+#pragma unroll
+                for (int np = 0; np < TILES / 2; ++np)
+                    stsm4_trans(values + np * 512, pack2(dy[2 * np][0], dy[2 * np][1]), pack2(dy[2 * np][2], dy[2 * np][3]),
+                                pack2(dy[2 * np + 1][0], dy[2 * np + 1][1]), pack2(dy[2 * np + 1][2], dy[2 * np + 1][3]));
+                __syncwarp();
+                const int count = min(CHUNK, length - c * CHUNK);
+                char* to = reinterpret_cast<char*>(dv_out + ((row + int64_t(c) * CHUNK) * shape.heads + head) * dv + column);
+#pragma unroll
+                for (int i = 0; i < CHUNK * 2 / 32; ++i) {
+                    const int t = i * 16 + (lane >> 1);
+                    const uint4 piece = *reinterpret_cast<const uint4*>(shared + Stage::X + warp * 2048 + t * 32 + (((lane & 1) ^ ((t >> 2) & 1)) * 16));
+                    if (t < count) *reinterpret_cast<uint4*>(to + t * value_stride + (lane & 1) * 16) = piece;
+                }
+                __syncwarp();  // the room is free for the next chunk's X
+            }
+            // scale e^G dO and -e^G dY, the left operands of the state's step
+#pragma unroll
+            for (int np = 0; np < TILES / 2; ++np) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float2 decay = *reinterpret_cast<const float2*>(rows + 16 * np + 8 * h + 2 * (lane & 3));
+                    const float sx = shape.scale * decay.x, sy = shape.scale * decay.y;
+                    float(&tile)[4] = dy[2 * np + h];
+                    tile[0] *= -decay.x, tile[1] *= -decay.y, tile[2] *= -decay.x, tile[3] *= -decay.y;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        grad[np][2 * h + e] = pack2(low_half(grad[np][2 * h + e]) * sx, high_half(grad[np][2 * h + e]) * sy);
+                }
+                to_operand(dx[np], dy[2 * np], dy[2 * np + 1]);
+            }
+            const float kept = rows[CHUNK - 1];
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ds[n][e] *= kept;
+            const TileLane keys_trans = tile_rows_first<Stage::PITCH>(stage + Stage::K, lane);
+#pragma unroll
+            for (int kb = 0; kb < TILES / 2; ++kb)
+#pragma unroll
+                for (int np = 0; np < D / 16; ++np) {
+                    unsigned b[4];
+                    ldsm4_trans(b, keys_trans.at(np * 32) + kb * 16 * Stage::PITCH);
+                    mma16816(ds[2 * np], dx[kb], b[0], b[1]);
+                    mma16816(ds[2 * np + 1], dx[kb], b[2], b[3]);
+                    ldsm4_trans(b, keys_trans.at(np * 32) + Stage::Q - Stage::K + kb * 16 * Stage::PITCH);
+                    mma16816(ds[2 * np], grad[kb], b[0], b[1]);
+                    mma16816(ds[2 * np + 1], grad[kb], b[2], b[3]);
+                }
+        }
+        if (LOCAL) {
+            float4* to = reinterpret_cast<float4*>(ends + (int64_t(part.segment) * shape.heads + head) * D * dv) + column / 16 * (D / 8) * 32 + lane;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) to[n * 32] = *reinterpret_cast<float4*>(ds[n]);
+        } else if (SHARES && part.to) {
+            float4* to = reinterpret_cast<float4*>(part.to) + warp * (D / 8) * 32 + lane;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) to[n * 32] = *reinterpret_cast<float4*>(ds[n]);
+        } else if (dinitial && number == 0) {
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    dinitial[state_at + int64_t(8 * n + 2 * (lane & 3) + (e & 1)) * dv + (e >> 1) * 8] = ds[n][e];
+        }
+        more = SHARES && share.next(part);
+    } while (more);
 }
 
 constexpr int GRADIENT_THREADS = 256;
@@ -608,8 +632,18 @@ cudaError_t launch_reverse(const DeltaShape& shape, const DeltaGradients& x, con
         if (shape.segments.length)
             if (cudaError_t status = launch_reverse<D, WARPS, true>(shape, x, saved, stream)) return status;
     constexpr int BYTES = ReverseStage<D, WARPS>::TOTAL;
-    constexpr auto* kernel = delta_reverse_kernel<D, WARPS, LOCAL>;
+    constexpr auto* kernel = delta_reverse_kernel<D, WARPS, LOCAL, false>;
     if (cudaError_t status = allow_shared<kernel>(BYTES)) return status;
+    if constexpr (!LOCAL && D >= 64 && WARPS == 4)
+        if (shape.shares.length) {
+            constexpr auto* shared_kernel = delta_reverse_kernel<D, WARPS, false, true>;
+            if (cudaError_t status = allow_shared<shared_kernel>(BYTES)) return status;
+            if (cudaError_t status = cudaMemsetAsync(shape.shares.flags, 0, shape.shares.flag_bytes(), stream)) return status;
+            KernelTimer timer("delta_reverse", stream);
+            shared_kernel<<<shape.shares.places, WARPS * 32, BYTES, stream>>>(shape, x.q, x.k, x.dout, x.dfinal, saved, x.dstates, x.dbeta_parts, x.dv,
+                                                                              x.dinitial, nullptr);
+            return cudaGetLastError();
+        }
     KernelTimer timer(LOCAL ? "delta_reverse_segments" : "delta_reverse", stream);
     kernel<<<dim3(unsigned(shape.segments.count(shape.layout)), shape.heads, shape.dv / (16 * WARPS)), WARPS * 32, BYTES, stream>>>(
         shape, x.q, x.k, x.dout, x.dfinal, saved, x.dstates, x.dbeta_parts, x.dv, x.dinitial, x.ends);
@@ -637,6 +671,12 @@ cudaError_t launch_width(const DeltaShape& shape, const DeltaGradients& x, const
     return launch_gradient<D, 128>(shape, x, saved, stream);
 }
 }  // namespace
+
+cudaError_t read_reverse_fault(int* code) {
+    if (cudaError_t status = cudaMemcpyFromSymbol(code, delta_reverse_fault, sizeof(int))) return status;
+    const int zero = 0;
+    return cudaMemcpyToSymbol(delta_reverse_fault, &zero, sizeof(int));
+}
 
 cudaError_t launch_delta_backward(const DeltaShape& shape, const DeltaGradients& x, const DeltaSaved& saved, cudaStream_t stream) {
     if (shape.d == 32) return launch_width<32>(shape, x, saved, stream);

@@ -172,12 +172,81 @@ struct DeltaSegments {
     }
 };
 
+// Chains of equal sequences that would leave the device partly empty at the end are walked in equal shares instead (length 0: they are not):
+// with all chains laid end to end, place i takes the chunks from i * length on.  A share is no shorter than a chain, so no more than
+// one chain is cut at its end; that one is walked first and its state, in 32 bits, handed to the next place, which walks the rest of it last.
+struct DeltaShares {
+    int length, places;
+    float* states;    // accumulator fragments, [places, D * 64]
+    unsigned* flags;  // tickets drawn; then one for each place: its state is there.  Zeros before the launch.
+    size_t flag_bytes() const { return size_t(places + 1) * 4; }
+};
+// What one walk covers: a segment (or sequence), value head and block of columns; with shares, chunks begin .. end - 1 in walking order,
+// from the state at `from` (null: the sequence's first) and leaving the state at `to` (null: the sequence ends).
+struct DeltaPart {
+    unsigned segment, head, block;
+    int begin, end;
+    const float* from;
+    float* to;
+};
+
 struct DeltaShape {
     DeltaLayout layout;
     DeltaSegments segments;
+    DeltaShares shares;
     int key_heads, heads, d, dv;
     bool gates_bf16;
     float scale;
+};
+
+// The parts of a CTA's share.  Places are drawn in the order in which CTAs start, so the one before has started, and what it hands on comes
+// first and waits for nobody: no wait depends on CTAs that are not resident.  It is bounded all the same, by about two seconds; then `code`
+// is recorded in `fault` and the walk goes on from whatever is there.  STATE: floats of a state that is handed on.
+template <int STATE>
+struct ShareWalk {
+    int64_t chain, lowest, highest;
+    int first, last, chunks;  // the lowest chain's first chunk, the end of the highest one's
+    unsigned blocks;
+    float* states;
+    unsigned* flag;
+    __device__ __forceinline__ bool draw(const DeltaShape& shape, unsigned columns) {  // false: more CTAs than places
+        __shared__ int drawn;
+        if (threadIdx.x == 0) drawn = int(atomicAdd(shape.shares.flags, 1u));
+        __syncthreads();
+        const int place = drawn;
+        chunks = shape.layout.chunks(), blocks = shape.dv / columns;
+        const int64_t all = int64_t(shape.layout.sequences) * shape.heads * blocks * chunks, begin = int64_t(place) * shape.shares.length;
+        const int64_t end = min(begin + shape.shares.length, all);
+        lowest = begin / chunks, highest = chain = (end - 1) / chunks;
+        first = int(begin - lowest * chunks), last = int(end - highest * chunks);
+        states = shape.shares.states + int64_t(place) * STATE, flag = shape.shares.flags + 1 + place;
+        return place < shape.shares.places;
+    }
+    __device__ __forceinline__ DeltaPart part(const DeltaShape& shape, int* fault, int code) const {
+        const int begin = chain == lowest ? first : 0, end = chain == highest ? last : chunks;
+        if (begin > 0) {
+            if (threadIdx.x == 0) {
+                unsigned there = 0;
+                for (int tries = 0; tries < 1 << 22 && !there; ++tries) {
+                    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(flag - 1) : "memory");
+                    if (!there) __nanosleep(500);
+                }
+                if (!there) atomicCAS(fault, 0, code);
+            }
+            __syncthreads();
+        }
+        const int64_t sequence = chain / blocks;
+        return DeltaPart{unsigned(sequence / shape.heads), unsigned(sequence % shape.heads), unsigned(chain % blocks), begin, end,
+                         begin > 0 ? states - STATE : nullptr, end < chunks ? states : nullptr};
+    }
+    __device__ __forceinline__ bool next(const DeltaPart& walked) {  // false: that was the last part
+        __syncthreads();  // the stages are free, and a state that is handed on is written
+        if (walked.to && threadIdx.x == 0) {
+            __threadfence();
+            asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(flag), "r"(1u) : "memory");
+        }
+        return --chain >= lowest;
+    }
 };
 
 // Zeros in the gradients' rows of no document; CTA `index` of `count` takes every count-th row.
@@ -277,6 +346,7 @@ __device__ __forceinline__ void load_block(unsigned tile, const char* global, in
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tile + i), "l"(global + i));
 }
 
+DeltaShares delta_shares(const DeltaLayout& layout, int heads, int d, int dv);
 // Chunks to a segment, 0 for whole sequences.
 int delta_segment_length(const DeltaLayout& layout, int heads, int d, int dv);
 struct DeltaGradients {
@@ -298,8 +368,10 @@ cudaError_t launch_delta_chain(const DeltaShape& shape, const __nv_bfloat16* q, 
 cudaError_t launch_delta_backward(const DeltaShape& shape, const DeltaGradients& gradients, const DeltaSaved& saved, cudaStream_t stream);
 // The last stage of the backward on tcgen05, for D and DV of 64 or 128.
 cudaError_t launch_delta_gradient_tensor(const DeltaShape& shape, const DeltaGradients& gradients, const DeltaSaved& saved, cudaStream_t stream);
-// First bounded wait of the tensor-memory pipeline that ran out on the current device, 0 if none; reading clears it.
+// First bounded wait that ran out on the current device, of the tensor-memory pipeline (1 to 10) or between shares (11, 12), 0 if none; reading clears it.
 cudaError_t read_delta_fault(int* code);
+cudaError_t read_chain_fault(int* code);
+cudaError_t read_reverse_fault(int* code);
 cudaError_t launch_delta_step(const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v, const void* g, const void* beta,
                               bool gates_bf16, float scale, float* state, const int* slots, int64_t pool, int batch, int key_heads,
                               int heads, int d, int dv, __nv_bfloat16* out, cudaStream_t stream);

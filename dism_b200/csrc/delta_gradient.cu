@@ -498,8 +498,12 @@ cudaError_t launch_delta_gradient_tensor(const DeltaShape& shape, const DeltaGra
 }
 
 cudaError_t read_delta_fault(int* code) {
-    if (cudaError_t status = cudaMemcpyFromSymbol(code, delta_gradient_fault, sizeof(int))) return status;
+    int chain = 0, reverse = 0;
     const int zero = 0;
+    if (cudaError_t status = read_chain_fault(&chain)) return status;
+    if (cudaError_t status = read_reverse_fault(&reverse)) return status;
+    if (cudaError_t status = cudaMemcpyFromSymbol(code, delta_gradient_fault, sizeof(int))) return status;
+    if (chain || reverse) *code = chain ? chain : reverse;  // the earlier stage
     return cudaMemcpyToSymbol(delta_gradient_fault, &zero, sizeof(int));
 }
 

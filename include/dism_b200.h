@@ -189,7 +189,7 @@ int dism_delta_backward(const void *q, const void *k, const void *dout, const fl
                         const void *saved, size_t saved_bytes, void *dq, void *dk, void *dv_out, void *dg, void *dbeta,
                         float *dinitial_state, void *workspace, size_t workspace_bytes, void *stream);
 
-/* The tensor-memory pipelines of the rule bound every wait; *code is the first that ran out on the current device since the last
+/* The kernels of the rule bound every wait (tensor-memory pipelines, and a CTA's for a state another one hands on); *code is the first that ran out on the current device since the last
  * call (0: none, the only value a correct run produces); the call clears it.  Synchronises the device. */
 int dism_delta_fault(int *code);
 

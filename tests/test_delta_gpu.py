@@ -322,6 +322,47 @@ def test_a_graph_can_be_walked_twice(flash, n, d):
     assert all(torch.equal(a, b) for a, b in zip(first, second))
 
 
+@pytest.mark.parametrize('batch,key_heads,heads,n,d,dv', [(150, 1, 2, 513, 64, 64), (75, 2, 2, 576, 128, 128), (298, 1, 2, 520, 64, 64), (100, 3, 3, 700, 128, 64), (149, 1, 1, 650, 64, 128)])
+def test_chains_in_shares(flash, batch, key_heads, heads, n, d, dv):
+    """More chains than fit at once are walked in equal shares: the same numbers as from parts of the batch, which fit; also captured, and
+    from two streams at once."""
+    room = 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    x = [t.cuda() for t in reference.operands(15, batch, n, key_heads, heads, d, dv)]
+    s0 = torch.randn(batch, heads, d, dv, device='cuda')
+    dout, dfinal = torch.randn_like(x[2]), torch.randn_like(s0)
+
+    def step(part, states=True):
+        leaves = [t[part].clone().requires_grad_() for t in (*x, s0)]
+        out = flash.gated_delta_rule(*leaves[:5], initial_state=leaves[5], output_final_state=states)
+        outs, grads = (out, (dout[part], dfinal[part])) if states else ((out,), (dout[part],))
+        return [*outs, *torch.autograd.grad(outs, leaves, grads)]
+    assert batch * heads * (dv // 64) > room or room != 296
+    for states in (True, False):
+        whole = step(slice(None), states)
+        third = (batch + 2) // 3
+        parts = [step(slice(i, i + third), states) for i in range(0, batch, third)]
+        assert all(torch.equal(a, torch.cat(b)) for a, b in zip(whole, zip(*parts)))
+        if states:
+            assert torch.equal(whole[0], flash.gated_delta_rule(*x, initial_state=s0, output_final_state=True)[0])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for stream in streams:
+        with torch.cuda.stream(stream):
+            got.append(flash.gated_delta_rule(*x, initial_state=s0))
+    torch.cuda.synchronize()
+    want = flash.gated_delta_rule(*x, initial_state=s0)
+    assert all(torch.equal(a, want) for a in got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = flash.gated_delta_rule(*x, initial_state=s0)
+    for _ in range(2):
+        captured.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, want)
+
+
 def test_two_calls_at_once(flash):
     """Two streams, each with its own call in flight many times over, do not disturb one another."""
     sets = [[t.cuda().requires_grad_() for t in reference.operands(s, 1, 500, 2, 2, 64, 64)] for s in (1, 2)]
