@@ -333,7 +333,7 @@ size_t lay_out_delta(dism::DeltaShape& shape, bool exact, bool backward, char* b
     }
     const size_t segments = shape.segments.length ? size_t(shape.segments.count(shape.layout)) * shape.heads : 0;
     shape.segments.m = reinterpret_cast<bf*>(take(segments * shape.d * shape.d * 2));
-    if (exact) shape.segments.m_rest = reinterpret_cast<bf*>(take(segments * shape.d * shape.d * 2));
+    shape.segments.m_rest = reinterpret_cast<bf*>(take(segments * shape.d * shape.d * 2));
     shape.segments.ends = reinterpret_cast<float*>(take(segments * shape.d * shape.dv * 4));
     if (exact) parts.t_rest = reinterpret_cast<bf*>(take(places * dism::MATRIX * 2));
     if (shape.shares.length) {

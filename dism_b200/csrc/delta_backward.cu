@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
 #pragma unroll
             for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float4*>(ds[n]) = __ldcg(from + n * 32);
         }
-        // the gradient behind an earlier segment: dS <- M^T dS + B over the segments behind it.  The last one's B already has dfinal.
+        // the gradient behind an earlier segment: dS <- M^T dS + B over the segments behind it, M and dS as pairs as in the forward.  The last one's B already has dfinal.
         if (!LOCAL && !SHARES)
             for (int later = behind; later > 0; --later) {
                 const int64_t place = (int64_t(part.segment) + later) * shape.heads + head;
@@ -113,17 +113,25 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
                 for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float4*>(x[n]) = __ldg(end + n * 32);
                 if (later < behind) {
                     load_block<2 * D * D, THREADS>(base, reinterpret_cast<const char*>(shape.segments.m + place * D * D), thread);
+                    load_block<2 * D * D, THREADS>(base + 2 * D * D, reinterpret_cast<const char*>(shape.segments.m_rest + place * D * D), thread);
                     cp_async_commit();
                     cp_async_wait<0>();
                     __syncthreads();
 #pragma unroll
                     for (int kb = 0; kb < D / 16; ++kb) {
-                        unsigned a[4];
+                        unsigned a[4], rest[4];
                         to_operand(a, ds[2 * kb], ds[2 * kb + 1]);
+                        to_operand_rest(rest, a, ds[2 * kb], ds[2 * kb + 1]);
+                        const unsigned m = base + kb * 2 * 128 + cols_first_blocked(lane, D / 8);
 #pragma unroll
                         for (int np = 0; np < D / 16; ++np) {
                             unsigned b[4];
-                            ldsm4(b, base + (np * 2 * (D / 8) + kb * 2) * 128 + cols_first_blocked(lane, D / 8));
+                            ldsm4(b, m + np * 2 * (D / 8) * 128);
+                            mma16816(x[2 * np], a, b[0], b[1]);
+                            mma16816(x[2 * np + 1], a, b[2], b[3]);
+                            mma16816(x[2 * np], rest, b[0], b[1]);
+                            mma16816(x[2 * np + 1], rest, b[2], b[3]);
+                            ldsm4(b, m + 2 * D * D + np * 2 * (D / 8) * 128);
                             mma16816(x[2 * np], a, b[0], b[1]);
                             mma16816(x[2 * np + 1], a, b[2], b[3]);
                         }

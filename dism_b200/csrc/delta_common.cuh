@@ -146,7 +146,7 @@ struct DeltaLayout {
 struct DeltaSegments {
     int length;
     float* ends;                  // B as accumulator fragments, [segments, H, D * DV]
-    __nv_bfloat16 *m, *m_rest;    // M, transposed, in 8 x 8 blocks, [segments, H, D * D]; the remainders only for an exact state
+    __nv_bfloat16 *m, *m_rest;    // M, transposed, in 8 x 8 blocks, as pairs, [segments, H, D * D]
     __host__ __device__ int64_t count(const DeltaLayout& layout) const {
         if (!length) return layout.sequences;
         if (!layout.cu) return int64_t(layout.sequences) * ((layout.chunks() + length - 1) / length);
