@@ -331,7 +331,7 @@ size_t lay_out_delta(dism::DeltaShape& shape, bool exact, bool backward, char* b
         parts.states = reinterpret_cast<bf*>(take(places * shape.d * shape.dv * 2));
         parts.x = reinterpret_cast<bf*>(take(places * dism::CHUNK * shape.dv * 2));
     }
-    const size_t segments = shape.segments.length ? size_t(shape.segments.count(shape.layout)) * shape.heads : 0;
+    const size_t segments = size_t(shape.segments.stored(shape.layout)) * shape.heads;
     shape.segments.m = reinterpret_cast<bf*>(take(segments * shape.d * shape.d * 2));
     shape.segments.m_rest = reinterpret_cast<bf*>(take(segments * shape.d * shape.d * 2));
     shape.segments.ends = reinterpret_cast<float*>(take(segments * shape.d * shape.dv * 4));
@@ -345,7 +345,7 @@ size_t lay_out_delta(dism::DeltaShape& shape, bool exact, bool backward, char* b
 }
 size_t delta_scratch(dism::DeltaShape& shape, char* base, dism::DeltaGradients* x) {
     const size_t places = size_t(shape.layout.slots()) * shape.heads;
-    const size_t segments = shape.segments.length ? size_t(shape.segments.count(shape.layout)) * shape.heads : 0;
+    const size_t segments = size_t(shape.segments.stored(shape.layout)) * shape.heads;
     const size_t states = round_up(places * shape.d * shape.dv * 2), parts = round_up(places * dism::CHUNK * (shape.dv / 16) * 4);
     const size_t ends = round_up(segments * shape.d * shape.dv * 4), shares = shape.shares.length ? round_up(size_t(shape.shares.places) * shape.d * dism::CHUNK * 4) : 0;
     if (x) {

@@ -106,8 +106,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
         // the gradient behind an earlier segment: dS <- M^T dS + B over the segments behind it, M and dS as pairs as in the forward.  The last one's B already has dfinal.
         if (!LOCAL && !SHARES)
             for (int later = behind; later > 0; --later) {
-                const int64_t place = (int64_t(part.segment) + later) * shape.heads + head;
-                const float4* end = reinterpret_cast<const float4*>(ends + place * D * dv) + column / 16 * (D / 8) * 32 + lane;
+                const int64_t place = (shape.segments.place(slot) + later) * shape.heads + head;  // of M; B lies one before
+                const float4* end = reinterpret_cast<const float4*>(ends + (place - shape.heads) * D * dv) + column / 16 * (D / 8) * 32 + lane;
                 float x[D / 8][4];
 #pragma unroll
                 for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float4*>(x[n]) = __ldg(end + n * 32);
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
                 }
         }
         if (LOCAL) {
-            float4* to = reinterpret_cast<float4*>(ends + (int64_t(part.segment) * shape.heads + head) * D * dv) + column / 16 * (D / 8) * 32 + lane;
+            float4* to = reinterpret_cast<float4*>(ends + ((shape.segments.place(slot) - 1) * shape.heads + head) * D * dv) + column / 16 * (D / 8) * 32 + lane;
 #pragma unroll
             for (int n = 0; n < D / 8; ++n) to[n * 32] = *reinterpret_cast<float4*>(ds[n]);
         } else if (SHARES && part.to) {

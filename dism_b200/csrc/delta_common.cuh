@@ -141,12 +141,17 @@ struct DeltaLayout {
 // A chain of chunks is cut into segments of `length` chunks (0: not cut) when there are too few chains to fill the device.  The state is
 // linear in the state at the segment's start, S_end = M S_start + B, so a first launch finds M (the chain applied to the unit matrix
 // without values) and B (the chain from zero) of all segments but the last of a sequence at once, and a second one runs every segment
-// from its true start, which it puts together from the M and B before it.  Segments are numbered like chunks: in a pack, document i
-// begins at segment slot / length + i.
+// from its true start, which it puts together from the M and B before it.  CTAs are numbered like chunks: in a pack, document i
+// begins at segment slot / length + i.  What is kept of segments lies closer: of a sequence of c chunks only the first (c - 1) / length segments
+// are (the last has no successor; in the reverse chain, the first no predecessor, and the others move up by one), so they fit from place
+// slot / length on without meeting the next sequence's, and short documents take no room.
 struct DeltaSegments {
     int length;
-    float* ends;                  // B as accumulator fragments, [segments, H, D * DV]
-    __nv_bfloat16 *m, *m_rest;    // M, transposed, in 8 x 8 blocks, as pairs, [segments, H, D * D]
+    float* ends;                  // B as accumulator fragments, [stored, H, D * DV]
+    __nv_bfloat16 *m, *m_rest;    // M, transposed, in 8 x 8 blocks, as pairs, [stored, H, D * D]
+    __host__ __device__ int64_t stored(const DeltaLayout& layout) const { return length ? layout.slots() / length : 0; }
+    // The place of the segment that begins with the chunk in this slot; that of the next one of the sequence is one further.
+    __device__ int64_t place(int64_t slot) const { return slot / length; }
     __host__ __device__ int64_t count(const DeltaLayout& layout) const {
         if (!length) return layout.sequences;
         if (!layout.cu) return int64_t(layout.sequences) * ((layout.chunks() + length - 1) / length);

@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
         // after 32 joins.
         if (!LOCAL && !SHARES)
             for (int before = 0; before < number; ++before) {
-                const int64_t place = (int64_t(part.segment) - number + before) * shape.heads + head;
+                const int64_t place = (shape.segments.place(slot) - number + before) * shape.heads + head;
                 load_block<2 * D * D, THREADS>(base, reinterpret_cast<const char*>(shape.segments.m + place * D * D), thread);
                 load_block<2 * D * D, THREADS>(base + 2 * D * D, reinterpret_cast<const char*>(shape.segments.m_rest + place * D * D), thread);
                 cp_async_commit();
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
                 }
         }
         if (LOCAL) {
-            const int64_t place = int64_t(part.segment) * shape.heads + head;
+            const int64_t place = shape.segments.place(slot) * shape.heads + head;
             if (unit) {
                 unsigned* to = reinterpret_cast<unsigned*>(shape.segments.m + place * D * D) + int64_t(column / 8) * (D / 8) * 32 + lane;
                 unsigned* to_rest = reinterpret_cast<unsigned*>(shape.segments.m_rest + place * D * D) + int64_t(column / 8) * (D / 8) * 32 + lane;

@@ -128,7 +128,7 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, output
     lengths), must ascend, and rows outside [cu_seqlens[0], cu_seqlens[-1]) come out as zeros.  initial_state is FP32
     [sequences,H,D,DV].  All operands and the initial state are differentiable; gates receive gradients in their own type, with
     the relative accuracy of the bf16 operands.  Keeping the states for a backward takes 2 D DV / 64 + 2 DV + 184 bytes per position
-    and head, and 4 D D + 4 D DV per segment and head where a long chain is cut, or 256 D
+    and head, and 4 D D + 4 D DV per segment and head where a long chain is cut (documents of a pack that are shorter than a segment add none), or 256 D
     per place of the device (two an SM) where chains are walked in shares."""
     starts = _documents(v, cu_seqlens, layout)
     needed = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad
