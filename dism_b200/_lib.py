@@ -37,6 +37,7 @@ SIGNATURES = {
     'dism_delta_backward_workspace': (_Z, [_I] * 6),
     'dism_delta_backward': (_I, [_P] * 4 + [_I, _P] + [_I] * 6 + [_c.c_float, _P, _Z] + [_P] * 7 + [_Z, _P]),
     'dism_delta_fault': (_I, [_P]),
+    'dism_delta_wait_limit': (_I, [_I]),
     'dism_delta_step': (_I, [_P] * 5 + [_I, _P, _P, _c.c_int64] + [_I] * 5 + [_c.c_float, _P, _P]),
     'dism_dropout': (_I, [_I, _P, _P, _c.c_int64, _I, _P, _c.c_uint32, _P, _P]),
     'dism_longest_match': (_I, [_P, _I, _I, _P, _P, _P, _P, _Z, _P]),

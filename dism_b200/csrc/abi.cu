@@ -3,6 +3,7 @@
 // so callers that match on them keep working.
 #include "../../include/dism_b200.h"
 #include "delta_common.cuh"
+#include "tensor_memory.cuh"
 
 #include <climits>
 #include <cstdarg>
@@ -93,7 +94,7 @@ int dism_profile_read(int index, char* name, int capacity, float* milliseconds) 
 }
 
 const char* dism_last_error(void) { return last_error; }
-int dism_abi_version(void) { return 10; }
+int dism_abi_version(void) { return 11; }
 
 int dism_route_word(const uint32_t* choice) {
     if (choice && !aligned(choice, 4)) return fail(DISM_EINVAL, "graph choice must be one aligned device int32");
@@ -312,6 +313,7 @@ static int check_delta(int packed, int sequences, int n, int key_heads, int head
 }
 
 namespace {
+std::atomic<unsigned> delta_wait_tries{dism::TM_WAIT_TRIES};
 constexpr size_t round_up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 // The parts of `saved`, in the order in which they lie; those that `exact` or `backward` do not ask for have no bytes.
 size_t lay_out_delta(dism::DeltaShape& shape, bool exact, bool backward, char* base, dism::DeltaSaved* saved) {
@@ -360,7 +362,8 @@ size_t delta_scratch(dism::DeltaShape& shape, char* base, dism::DeltaGradients* 
 dism::DeltaShape delta_shape(const int32_t* cu_seqlens, int sequences, int n, int key_heads, int heads, int d, int dv, int gates_bf16, float scale) {
     const dism::DeltaLayout layout{cu_seqlens, sequences, n};
     return dism::DeltaShape{layout, dism::DeltaSegments{dism::delta_segment_length(layout, heads, d, dv), nullptr, nullptr, nullptr},
-                            dism::delta_shares(layout, heads, d, dv), key_heads, heads, d, dv, gates_bf16 != 0, scale};
+                            dism::delta_shares(layout, heads, d, dv), key_heads, heads, d, dv, gates_bf16 != 0, scale,
+                            delta_wait_tries.load(std::memory_order_relaxed)};
 }
 }  // namespace
 
@@ -420,6 +423,12 @@ int dism_delta_backward(const void* q, const void* k, const void* dout, const fl
 int dism_delta_fault(int* code) {
     if (!code) return fail(DISM_EINVAL, "null pointer");
     return cuda_status(dism::read_delta_fault(code), "delta fault code");
+}
+
+int dism_delta_wait_limit(int tries) {
+    if (tries > int(dism::TM_WAIT_TRIES)) return fail(DISM_EINVAL, "at most %u tries", dism::TM_WAIT_TRIES);
+    delta_wait_tries.store(tries < 0 ? dism::TM_WAIT_TRIES : unsigned(tries), std::memory_order_relaxed);
+    return DISM_OK;
 }
 
 int dism_delta_step(const void* q, const void* k, const void* v, const void* g, const void* beta, int gates_bf16, float* state,

@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
     if (SHARES && !share.draw(shape, WARPS * 16)) return;
     bool more = false;
     do {
-        const DeltaPart part = SHARES ? share.part(shape, &delta_reverse_fault, 12) : DeltaPart{blockIdx.x, blockIdx.y, blockIdx.z, 0, 0, nullptr, nullptr};
+        const DeltaPart part = SHARES ? share.part(shape, &delta_reverse_fault, 13) : DeltaPart{blockIdx.x, blockIdx.y, blockIdx.z, 0, 0, nullptr, nullptr, false};
         const int head = part.head, dv = shape.dv;
         const int key_head = head / (shape.heads / shape.key_heads), column = (part.block * WARPS + warp) * 16;
         int64_t row, slot;
@@ -101,7 +101,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
         if (SHARES && part.from) {
             const float4* from = reinterpret_cast<const float4*>(part.from) + warp * (D / 8) * 32 + lane;
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float4*>(ds[n]) = __ldcg(from + n * 32);
+            for (int n = 0; n < D / 8; ++n)
+                *reinterpret_cast<float4*>(ds[n]) = part.lost ? make_float4(NOT_A_NUMBER, NOT_A_NUMBER, NOT_A_NUMBER, NOT_A_NUMBER) : __ldcg(from + n * 32);
         }
         // the gradient behind an earlier segment: dS <- M^T dS + B over the segments behind it, M and dS as pairs as in the forward.  The last one's B already has dfinal.
         if (!LOCAL && !SHARES)

@@ -39,6 +39,7 @@ constexpr int CHUNK = 64;
 constexpr int ROW_DECAY = 0, ROW_BETA = CHUNK, ROW_TAIL = 2 * CHUNK, ROW_WRITE = 3 * CHUNK, ROW_HIGH = 4 * CHUNK, ROW_LOW = 5 * CHUNK, ROW_VALUES = 6 * CHUNK;
 constexpr int MATRIX = 10 * 256;           // elements of T and P of one chunk and head: the 16 x 16 tiles up to the diagonal
 constexpr float LOG2E = 1.4426950408889634f;
+#define NOT_A_NUMBER __int_as_float(0x7fc00000)
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -193,6 +194,7 @@ struct DeltaPart {
     int begin, end;
     const float* from;
     float* to;
+    bool lost;  // what stands at `from` was not waited for
 };
 
 struct DeltaShape {
@@ -202,11 +204,12 @@ struct DeltaShape {
     int key_heads, heads, d, dv;
     bool gates_bf16;
     float scale;
+    unsigned wait_tries;  // limit of the bounded waits: polls of a barrier, by up to 20 microseconds each; 64 times as many of a share's flag
 };
 
 // The parts of a CTA's share.  Places are drawn in the order in which CTAs start, so the one before has started, and what it hands on comes
 // first and waits for nobody: no wait depends on CTAs that are not resident.  It is bounded all the same, by about two seconds; then `code`
-// is recorded in `fault` and the walk goes on from whatever is there.  STATE: floats of a state that is handed on.
+// is recorded in `fault` and the walk goes on from a state of NaN.  STATE: floats of a state that is handed on.
 template <int STATE>
 struct ShareWalk {
     int64_t chain, lowest, highest;
@@ -229,20 +232,21 @@ struct ShareWalk {
     }
     __device__ __forceinline__ DeltaPart part(const DeltaShape& shape, int* fault, int code) const {
         const int begin = chain == lowest ? first : 0, end = chain == highest ? last : chunks;
+        bool lost = false;
         if (begin > 0) {
+            unsigned there = threadIdx.x;
             if (threadIdx.x == 0) {
-                unsigned there = 0;
-                for (int tries = 0; tries < 1 << 22 && !there; ++tries) {
+                for (unsigned tries = 0; tries < 64 * shape.wait_tries && !there; ++tries) {
                     asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(flag - 1) : "memory");
                     if (!there) __nanosleep(500);
                 }
                 if (!there) atomicCAS(fault, 0, code);
             }
-            __syncthreads();
+            lost = __syncthreads_or(!there);
         }
         const int64_t sequence = chain / blocks;
         return DeltaPart{unsigned(sequence / shape.heads), unsigned(sequence % shape.heads), unsigned(chain % blocks), begin, end,
-                         begin > 0 ? states - STATE : nullptr, end < chunks ? states : nullptr};
+                         begin > 0 ? states - STATE : nullptr, end < chunks ? states : nullptr, lost};
     }
     __device__ __forceinline__ bool next(const DeltaPart& walked) {  // false: that was the last part
         __syncthreads();  // the stages are free, and a state that is handed on is written
@@ -373,7 +377,7 @@ cudaError_t launch_delta_chain(const DeltaShape& shape, const __nv_bfloat16* q, 
 cudaError_t launch_delta_backward(const DeltaShape& shape, const DeltaGradients& gradients, const DeltaSaved& saved, cudaStream_t stream);
 // The last stage of the backward on tcgen05, for D and DV of 64 or 128.
 cudaError_t launch_delta_gradient_tensor(const DeltaShape& shape, const DeltaGradients& gradients, const DeltaSaved& saved, cudaStream_t stream);
-// First bounded wait that ran out on the current device, of the tensor-memory pipeline (1 to 10) or between shares (11, 12), 0 if none; reading clears it.
+// First bounded wait that ran out on the current device, of the tensor-memory pipeline (1 to 11) or between shares (12, 13), 0 if none; reading clears it.
 cudaError_t read_delta_fault(int* code);
 cudaError_t read_chain_fault(int* code);
 cudaError_t read_reverse_fault(int* code);

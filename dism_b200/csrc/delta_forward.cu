@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
     if (SHARES && !share.draw(shape, WARPS * 16)) return;
     bool more = false;
     do {
-        const DeltaPart part = SHARES ? share.part(shape, &delta_chain_fault, 11) : DeltaPart{blockIdx.x, blockIdx.y, blockIdx.z, 0, 0, nullptr, nullptr};
+        const DeltaPart part = SHARES ? share.part(shape, &delta_chain_fault, 12) : DeltaPart{blockIdx.x, blockIdx.y, blockIdx.z, 0, 0, nullptr, nullptr, false};
         const int head = part.head, dv = shape.dv, key_head = head / (shape.heads / shape.key_heads);
         const bool unit = LOCAL && part.block * WARPS * 16 >= dv;  // this CTA's columns are the unit matrix's
         const int column = (part.block * WARPS + warp) * 16 - (unit ? dv : 0);
@@ -110,7 +110,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
         if (SHARES && part.from) {
             const float4* from = reinterpret_cast<const float4*>(part.from) + warp * (D / 8) * 32 + lane;
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float4*>(s[n]) = __ldcg(from + n * 32);
+            for (int n = 0; n < D / 8; ++n)
+                *reinterpret_cast<float4*>(s[n]) = part.lost ? make_float4(NOT_A_NUMBER, NOT_A_NUMBER, NOT_A_NUMBER, NOT_A_NUMBER) : __ldcg(from + n * 32);
         }
         // The state at a later segment's start: S <- M S + B over the segments before it.  M and S are pairs here whatever is wanted at the end: a
         // rounding at a join stays in the state, and with slow decays and weak writes (M close to one) single bf16 left 1.1 to 2.2 % of the output's norm

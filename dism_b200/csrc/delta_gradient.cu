@@ -141,12 +141,14 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
     tm_fence_after();
     volatile int* abort = &control.abort;
     const uint32_t tensor = control.tensor_memory;
-    auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return tm_wait(bar, parity, abort, &delta_gradient_fault, code); };
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return tm_wait(bar, parity, abort, &delta_gradient_fault, code, shape.wait_tries); };
     auto rows_of = [&](int item) { return reinterpret_cast<const float*>(shared + Tiles::ROWS + (item & 1) * ROW_VALUES * 4); };
     auto sums_of = [&](int item) { return reinterpret_cast<float*>(shared + Tiles::SUMS) + (item & 1) * Tiles::SUM_VALUES; };
     // 168 registers a thread at launch: the rows take 208, issue and loads 80
     if (warp >= WORK_WARPS) {
         tm_fewer_registers<80>();
+        uint64_t* flight = nullptr;  // the barrier of the role's last copies or products
+        uint32_t flight_parity = 0;
         if (warp == MMA_WARP) {
             for (int item = 0, keys = 0; items.valid(); ++item) {
                 const uint32_t qk_tile = base + Tiles::QK + keys * (D / 64 * STACK);
@@ -179,6 +181,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                     tm_commit(&control.first);
                 }
                 __syncwarp();
+                flight = &control.first, flight_parity = item & 1;
                 if (!__all_sync(FULL, wait(&control.pairs, item & 1, 4))) break;
                 tm_fence_after();
                 if (tm_elect()) {
@@ -196,6 +199,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                     tm_commit(&control.second);
                 }
                 __syncwarp();
+                flight = &control.second;
                 if (items.last_head(shape)) keys ^= 1;
                 items.next(shape);
             }
@@ -223,6 +227,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                     }
                 }
                 __syncwarp();
+                flight = boxes, flight_parity = (partial ? tails : item >> 1) & 1;
                 if (partial) {  // the rows behind a chunk that ends inside its tile are another document's
                     if (!__all_sync(FULL, wait(&control.tail, tails & 1, 10))) break;
                     ++tails;
@@ -243,6 +248,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                     tm_copy(base + Tiles::ROWS + (item & 1) * ROW_VALUES * 4, saved.rows + place * ROW_VALUES, ROW_VALUES * 4, loaded);
                 }
                 __syncwarp();
+                flight = loaded, flight_parity = (item >> 1) & 1;
                 if (items.last_head(shape)) keys ^= 1;
                 items.next(shape);
             }
@@ -258,8 +264,9 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                     const float2 x = __ldg(reinterpret_cast<const float2*>(dbeta_parts + i * stride + place * CHUNK) + lane);
                     parts[0][i] = x.x, parts[1][i] = x.y;
                 }
-                wait(&control.loaded[item & 1], (item >> 1) & 1, 4);
+                wait(&control.loaded[item & 1], (item >> 1) & 1, 11);
                 wait(&control.done[item & 1], (item >> 1) & 1, 6);
+                const bool lost = *abort;
                 {
                     float here[2], last = 0.f;
 #pragma unroll
@@ -275,6 +282,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
 #pragma unroll
                         for (int i = 0; i < DV / 16; ++i) b += parts[e][i];
                         b += sums[Tiles::COLUMN_SUM + 2 * CHUNK + p] + sums[Tiles::COLUMN_SUM + 3 * CHUNK + p];
+                        if (lost) b = NOT_A_NUMBER;
                         if (p < items.count) {
                             const int64_t index = (items.row + p) * shape.heads + head;
                             if (shape.gates_bf16) static_cast<__nv_bfloat16*>(dbeta)[index] = __float2bfloat16(b);
@@ -304,7 +312,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                             // a decay that is zero in 32 bits has no gradient; the sum would leave the roundings of terms that cancel
                             const float *high = rows + ROW_HIGH, *low = rows + ROW_LOW;
                             const float step = p ? (high[p] - high[p - 1]) + (low[p] - low[p - 1]) : high[0];
-                            const float x = step < -149.f ? 0.f : after + here[e];
+                            const float x = lost ? NOT_A_NUMBER : step < -149.f ? 0.f : after + here[e];
                             if (shape.gates_bf16) static_cast<__nv_bfloat16*>(dg)[index] = __float2bfloat16(x);
                             else static_cast<float*>(dg)[index] = x;
                         }
@@ -315,6 +323,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                 items.next(shape);
             }
         }
+        if (flight) tm_settle(flight, flight_parity);
     } else {
         tm_more_registers<208>();
         // this thread's row of tensor memory: position t, a query's (part 0) or a key's (part 1); its half of the columns
@@ -337,6 +346,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
             // dP~ or dL~ of this row: columns 32 half .. 32 half + 31
             {
                 const float high = rows[ROW_HIGH + t], low = rows[ROW_LOW + t];
+                const bool lost = *abort;  // then another warp may still have its rows of the last item in the room of the pairs
                 float row_sum = 0.f;
 #pragma unroll 1
                 for (int j = 32 * half; j < 32 * half + 32; j += 16) {
@@ -358,7 +368,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
                         row_sum += __fmul_rn(beta[i], y[i]);  // as the column sums have it: a pair that cancels in dG is one number
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; i += 8)
+                    for (int i = 0; i < 16 && !lost; i += 8)
                         *reinterpret_cast<uint4*>(shared + Tiles::PAIRS + r * 128 + ((((j + i) / 8) ^ (r & 7)) * 16)) =
                             make_uint4(pack2(z[i], z[i + 1]), pack2(z[i + 2], z[i + 3]), pack2(z[i + 4], z[i + 5]), pack2(z[i + 6], z[i + 7]));
                     const float column = transposing_sum(y, lane);
@@ -386,7 +396,7 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
             wait(&control.second, item & 1, 9);
             tm_fence_after();
             {
-                const float decay = rows[ROW_DECAY + t], f1 = part ? -decay : shape.scale * decay, f2 = rows[ROW_WRITE + t];
+                const float decay = rows[ROW_DECAY + t], f1 = *abort ? NOT_A_NUMBER : part ? -decay : shape.scale * decay, f2 = rows[ROW_WRITE + t];
                 float state_sum = 0.f, last_sum = 0.f;
                 const unsigned char* own = shared + Tiles::QK + keys * (D / 64 * STACK) + (half * COLUMNS >> 6) * STACK + r * 128;  // the row of Q or K
                 constexpr int ROW = 2 * COLUMNS, PIECES = ROW / 16;
@@ -462,7 +472,6 @@ __global__ void __launch_bounds__(GRADIENT_THREADS, 1) delta_gradient_tensor_ker
         }
     }
     __syncthreads();
-    if (control.abort) __nanosleep(1000000);  // copies and products in flight end before their memory is given back
     if (warp == 0) {
         tm_fence_after();
         tm_free(tensor, TM_COLUMNS);
@@ -500,6 +509,7 @@ cudaError_t launch_delta_gradient_tensor(const DeltaShape& shape, const DeltaGra
 cudaError_t read_delta_fault(int* code) {
     int chain = 0, reverse = 0;
     const int zero = 0;
+    if (cudaError_t status = cudaDeviceSynchronize()) return status;  // the copies alone wait for no non-blocking stream
     if (cudaError_t status = read_chain_fault(&chain)) return status;
     if (cudaError_t status = read_reverse_fault(&reverse)) return status;
     if (cudaError_t status = cudaMemcpyFromSymbol(code, delta_gradient_fault, sizeof(int))) return status;

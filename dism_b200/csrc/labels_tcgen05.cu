@@ -780,7 +780,9 @@ cudaError_t launch_labels_tcgen05(const __nv_bfloat16* x, const __nv_bfloat16* c
 
 // First bounded wait that ran out in any earlier launch on this device (0: none).  Synchronises the device.
 cudaError_t read_labels_fault(int* code) {
-    const cudaError_t status = cudaMemcpyFromSymbol(code, labels_fault_code, sizeof(int));
+    cudaError_t status = cudaDeviceSynchronize();  // the copy alone waits for no non-blocking stream
+    if (status != cudaSuccess) return status;
+    status = cudaMemcpyFromSymbol(code, labels_fault_code, sizeof(int));
     if (status != cudaSuccess) return status;
     const int none = 0;
     return cudaMemcpyToSymbol(labels_fault_code, &none, sizeof(int));  // read and clear

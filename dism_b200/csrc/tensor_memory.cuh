@@ -12,7 +12,8 @@
 namespace dism {
 
 // Every wait is bounded, by about a second.  When one runs out, `abort` is set, the code is recorded and every later wait of the CTA
-// returns at once: all roles run to their ends with whatever the buffers hold, no product is issued any more, tensor memory is freed.
+// returns at once: no copy or product is issued any more, those in flight are waited for (tm_settle), the other roles run to their ends
+// and write NaN, tensor memory is freed.  Whoever has passed a wait of the CTA after another role gave up sees `abort` set.
 constexpr unsigned TM_WAIT_TRIES = 1u << 16, TM_PARK_NANOSECONDS = 20000;
 
 __device__ __forceinline__ uint32_t tm_address(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
@@ -30,14 +31,19 @@ __device__ __forceinline__ bool tm_test_parked(uint64_t* bar, uint32_t parity) {
     return done != 0;
 }
 // False: this wait ran out or another role's did.
-__device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* fault, int code) {
-    for (unsigned tries = 0; tries < TM_WAIT_TRIES; ++tries) {
+__device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* fault, int code, unsigned limit) {
+    for (unsigned tries = 0; tries < limit; ++tries) {
         if (tm_test_parked(bar, parity)) return true;
         if (*abort) return false;
     }
     *abort = 1;
     atomicCAS(fault, 0, code);
     return false;
+}
+// What the role itself has in flight lands before its memory is given back: bounded like any wait, whatever has happened.
+__device__ __forceinline__ void tm_settle(uint64_t* bar, uint32_t parity) {
+    for (unsigned tries = 0; tries < TM_WAIT_TRIES; ++tries)
+        if (tm_test_parked(bar, parity)) return;
 }
 
 // Contiguous bytes (a multiple of 16, both addresses 16-byte aligned) into shared memory; the barrier counts them.

@@ -18,6 +18,7 @@ Beyond the reference's module: labels, labels_pair, longest_match, the gated del
 delta_step) and dropout.
 """
 import contextlib
+import ctypes
 import functools
 
 import torch
@@ -629,6 +630,15 @@ def delta_step(x, scale, state, slots=None):
         elif batch:
             out.zero_()
     return out
+
+
+def delta_fault(device=None):
+    """The first wait of the rule's kernels that ran out on a device since the last call, 0 if none did; waits for the device.
+    Outputs that such a wait was to bring are NaN."""
+    code = ctypes.c_int()
+    with torch.cuda.device(device):
+        _lib.check(_abi.dism_delta_fault(ctypes.byref(code)))
+    return code.value
 
 
 # ---- dropout ---------------------------------------------------------------------------------------

@@ -190,8 +190,12 @@ int dism_delta_backward(const void *q, const void *k, const void *dout, const fl
                         float *dinitial_state, void *workspace, size_t workspace_bytes, void *stream);
 
 /* The kernels of the rule bound every wait (tensor-memory pipelines, and a CTA's for a state another one hands on); *code is the first that ran out on the current device since the last
- * call (0: none, the only value a correct run produces); the call clears it.  Synchronises the device. */
+ * call (0: none, the only value a correct run produces); the call clears it.  Synchronises the device.  What a wait that
+ * ran out was to bring is NaN in the outputs, and so is all that follows from it. */
 int dism_delta_fault(int *code);
+/* Limits the waits of all later calls to `tries` polls (of up to 20 microseconds; negative: the default of 65536, which is also the
+ * most).  0 makes every wait run out at once: what a test of that path sets. */
+int dism_delta_wait_limit(int tries);
 
 /* One token per row, state updated in place: q, k bf16 [batch,HK,D], v, out bf16 [batch,H,DV], g, beta [batch,H],
  * state float [pool,H,D,DV].  slots device int32 [batch]: the state of each row, or NULL for state i at row i.  A slot outside
