@@ -87,7 +87,8 @@ def _host_starts(starts, device):
     if cached is None:
         if len(_starts) >= 32:
             _starts.pop(next(iter(_starts)), None)
-        cached = _starts[key] = torch.tensor(starts, dtype=torch.int32).to(device)
+        with torch.inference_mode(False):  # a training call may save what an evaluation has uploaded
+            cached = _starts[key] = torch.tensor(starts, dtype=torch.int32).to(device)
     if device.type == 'cuda':
         cached.record_stream(torch.cuda.current_stream(device))  # dropped, its memory waits for this call's kernels
     return cached

@@ -71,3 +71,14 @@ def test_short_documents_take_no_room_for_segments():
     assert lib.dism_delta_saved(1, 4096, 262144, 16, 128, 128, 1, 0) <= 1.03 * places * (384 * 4 + 3 * 2560 * 2)
     assert lib.dism_delta_saved(1, 4096, 262144, 16, 128, 128, 0, 1) <= 1.03 * places * (384 * 4 + 2 * 2560 * 2 + 128 * 128 * 2 + 64 * 128 * 2)
     assert lib.dism_delta_backward_workspace(1, 4096, 262144, 16, 128, 128) <= 1.03 * places * (128 * 128 * 2 + 64 * 8 * 4)
+
+
+def test_a_pack_seen_in_inference_mode_trains_afterwards(flash):
+    x = [t.cuda() for t in reference.operands(2, 1, 90, 1, 1, 32, 32)]
+    starts = torch.tensor([0, 33, 90], dtype=torch.int32)
+    with torch.inference_mode():
+        quiet = flash.gated_delta_rule(*x, cu_seqlens=starts)
+    leaves = [t.requires_grad_() for t in x]
+    out = flash.gated_delta_rule(*leaves, cu_seqlens=starts)
+    assert torch.equal(out, quiet)
+    assert all(torch.isfinite(t).all() for t in torch.autograd.grad(out, leaves, torch.ones_like(out)))
