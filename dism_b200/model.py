@@ -14,6 +14,7 @@ Chosen layers can be gated delta layers instead, as in the reference's hybrid (d
 decode one token at a time from a state, and both branches of a block can pass through residual dropout.
 """
 import math
+import operator
 
 import torch
 import torch.nn as nn
@@ -127,7 +128,10 @@ class DismLM(nn.Module):
         super().__init__()
         self.heads, self.head_dim, self.rope_base, self.dropout = heads, head_dim, rope_base, dropout
         self.embed = nn.Embedding(vocab, width)
-        self.blocks = nn.ModuleList(Block(width, heads, head_dim, DeltaLayer if i in set(delta_layers) else DismLayer) for i in range(depth))
+        delta_layers = {operator.index(i) for i in delta_layers}
+        if not delta_layers <= set(range(depth)):
+            raise ValueError(f'delta_layers must name blocks 0 to {depth - 1}')
+        self.blocks = nn.ModuleList(Block(width, heads, head_dim, DeltaLayer if i in delta_layers else DismLayer) for i in range(depth))
         if dropout:
             self.register_buffer('dropout_seed', torch.randint(0, 1 << 62, (2,)) * torch.tensor([1, 0]), persistent=False)
         self.unembed = nn.Linear(width, vocab, bias=False)

@@ -24,3 +24,18 @@ def test_starts_first_uploaded_in_inference_mode_serve_a_training_call():
     with torch.inference_mode():
         first = delta._host_starts([0, 21, 64], torch.device('cpu'))
     assert not first.is_inference() and delta._host_starts([0, 21, 64], torch.device('cpu')) is first
+
+
+def test_delta_layers_from_an_iterator_and_outside_the_model():
+    import pytest
+    import torch
+    from dism_b200.model import DeltaLayer, DismLM
+    make = lambda layers: DismLM(depth=4, width=64, heads=2, head_dim=32, vocab=64, delta_layers=layers)
+    with torch.device('meta'):
+        for layers in ((1, 3), (i for i in (1, 3)), range(1, 4, 2), {3, 1}):
+            assert [type(b.mixer) is DeltaLayer for b in make(layers).blocks] == [False, True, False, True]
+        for layers in ((4,), (-1,), (0, 9)):
+            with pytest.raises(ValueError, match='delta_layers'):
+                make(layers)
+        with pytest.raises(TypeError):
+            make((1.5,))
