@@ -154,14 +154,16 @@ class DismLM(nn.Module):
             return logits
         return F.cross_entropy(logits.float().view(-1, logits.size(-1)), targets.reshape(-1))
 
-    def _recurrent(self):
+    def _recurrent(self, states):
         if not all(isinstance(block.mixer, DeltaLayer) for block in self.blocks):
             raise NotImplementedError('DISM layers have no state to decode from; only a model of delta layers steps token by token')
+        if states is not None and len(states) != len(self.blocks):
+            raise ValueError('one state per block required')
 
     @torch.no_grad()
     def prefill(self, tokens, states=None):
         """tokens [B,N] -> (logits of the last position [B,vocab], one FP32 state [B,H,D,D] per block); `states` continues earlier ones."""
-        self._recurrent()
+        self._recurrent(states)
         x, after = rms(self.embed(tokens)), []
         for index, block in enumerate(self.blocks):
             y, state = block.mixer.prefill(rms(x), None if states is None else states[index])
@@ -172,7 +174,7 @@ class DismLM(nn.Module):
     @torch.no_grad()
     def step(self, tokens, states, slots=None):
         """One token per row, tokens [B] -> logits [B,vocab]; the states are updated in place (`slots`: int32 [B], each row's state)."""
-        self._recurrent()
+        self._recurrent(states)
         x = rms(self.embed(tokens))
         for block, state in zip(self.blocks, states):
             x = x + block.mixer.step(rms(x), state, slots)

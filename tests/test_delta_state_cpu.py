@@ -39,3 +39,16 @@ def test_delta_layers_from_an_iterator_and_outside_the_model():
                 make(layers)
         with pytest.raises(TypeError):
             make((1.5,))
+
+
+def test_states_have_to_be_one_per_block():
+    import pytest
+    import torch
+    from dism_b200.model import DismLM
+    model = DismLM(depth=3, width=64, heads=2, head_dim=32, vocab=64, delta_layers=range(3))
+    states = [torch.zeros(1, 2, 32, 32) for _ in range(4)]
+    for some in (states[:2], states, []):
+        with pytest.raises(ValueError, match='one state per block'):
+            model.step(torch.zeros(1, dtype=torch.long), some)
+        with pytest.raises(ValueError, match='one state per block'):
+            model.prefill(torch.zeros(1, 4, dtype=torch.long), some)
