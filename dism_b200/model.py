@@ -121,20 +121,30 @@ class DismLM(nn.Module):
 
     `delta_layers` names the blocks (by index) whose mixer is a DeltaLayer, the others are DISM layers.  `dropout` is the probability of
     residual dropout while training; its masks follow the buffer `dropout_seed`, int64 (key, offset), whose offset the program
-    advances once a step (model.dropout_seed[1] += 1, after the backward pass).  A model of delta layers only also runs
+    advances once a step (model.dropout_seed[1] += 1, after the backward pass) and which checkpoints hold.  Data-parallel replicas, whose
+    buffers may be one rank's, each set `dropout_rank` to draw masks of their own.  A model of delta layers only also runs
     from states: prefill() a prompt, then step() token by token."""
 
-    def __init__(self, depth=20, width=1280, heads=10, head_dim=128, vocab=65536, rope_base=100000., delta_layers=(), dropout=0.):
+    def __init__(self, depth=20, width=1280, heads=10, head_dim=128, vocab=65536, rope_base=100000., delta_layers=(), dropout=0.,
+                 dropout_rank=0):
         super().__init__()
-        self.heads, self.head_dim, self.rope_base, self.dropout = heads, head_dim, rope_base, dropout
+        self.heads, self.head_dim, self.rope_base, self.dropout, self.dropout_rank = heads, head_dim, rope_base, dropout, dropout_rank
         self.embed = nn.Embedding(vocab, width)
         delta_layers = {operator.index(i) for i in delta_layers}
         if not delta_layers <= set(range(depth)):
             raise ValueError(f'delta_layers must name blocks 0 to {depth - 1}')
         self.blocks = nn.ModuleList(Block(width, heads, head_dim, DeltaLayer if i in delta_layers else DismLayer) for i in range(depth))
         if dropout:
-            self.register_buffer('dropout_seed', torch.randint(0, 1 << 62, (2,)) * torch.tensor([1, 0]), persistent=False)
+            self.register_buffer('dropout_seed', torch.randint(0, 1 << 62, (2,)) * torch.tensor([1, 0]))
         self.unembed = nn.Linear(width, vocab, bias=False)
+
+    def _load_from_state_dict(self, state_dict, prefix, *rest):
+        # weights go from a model with dropout to one without and back
+        if self.dropout:
+            state_dict.setdefault(prefix + 'dropout_seed', self.dropout_seed)
+        else:
+            state_dict.pop(prefix + 'dropout_seed', None)
+        super()._load_from_state_dict(state_dict, prefix, *rest)
 
     def angles(self, n, device, dtype):
         inverse = 1. / self.rope_base ** (torch.arange(0, self.head_dim, 2, device=device, dtype=torch.float32) / self.head_dim)
@@ -148,7 +158,7 @@ class DismLM(nn.Module):
         hard = torch.ones(b, self.heads, dtype=torch.bool, device=x.device)
         p, seed = (self.dropout, self.dropout_seed) if self.dropout and self.training else (0., None)
         for index, block in enumerate(self.blocks):
-            x = block(x, cos, sin, hard, p, seed, 2 * index)
+            x = block(x, cos, sin, hard, p, seed, 2 * (index + self.dropout_rank * len(self.blocks)))
         logits = self.unembed(rms(x))
         if targets is None:
             return logits

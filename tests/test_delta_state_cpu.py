@@ -52,3 +52,24 @@ def test_states_have_to_be_one_per_block():
             model.step(torch.zeros(1, dtype=torch.long), some)
         with pytest.raises(ValueError, match='one state per block'):
             model.prefill(torch.zeros(1, 4, dtype=torch.long), some)
+
+
+def test_checkpoints_hold_the_masks_key_and_offset():
+    import torch
+    from dism_b200.model import DismLM
+    make = lambda p: DismLM(depth=1, width=64, heads=2, head_dim=32, vocab=64, delta_layers=(0,), dropout=p)
+    trained, resumed = make(.1), make(.1)
+    trained.dropout_seed[1] += 7
+    assert not torch.equal(trained.dropout_seed, resumed.dropout_seed)
+    resumed.load_state_dict(trained.state_dict())
+    assert torch.equal(trained.dropout_seed, resumed.dropout_seed) and resumed.dropout_seed.dtype == torch.int64
+    assert torch.equal(trained.bfloat16().dropout_seed, resumed.dropout_seed)
+    # with and without dropout, either way round: the weights are the same model's
+    quiet = make(0.)
+    quiet.load_state_dict(trained.state_dict())
+    other = make(.2)
+    before = other.dropout_seed.clone()
+    other.load_state_dict(quiet.state_dict())
+    assert torch.equal(other.dropout_seed, before) and 'dropout_seed' not in quiet.state_dict()
+    holder = torch.nn.ModuleDict(dict(m=make(0.)))
+    holder.load_state_dict({f'm.{k}': t for k, t in trained.state_dict().items()})
