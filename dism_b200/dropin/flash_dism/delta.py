@@ -146,7 +146,8 @@ def gated_delta_step(q, k, v, g, beta, state, *, scale=None, slots=None):
     row (default: state i for row i); a slot outside the pool marks a padding row, whose output is zero, and rows that name
     one slot are consecutive tokens of that sequence, in row order.  Everything is computed in 32 bits; not differentiable."""
     gates = _gate_type(g, beta)
-    if torch.is_tensor(state) and not state.is_inference():
-        torch.autograd.graph.increment_version(state)  # a graph that has saved the state sees that it changes
-    return cu.delta_step((_ready(q), _ready(k), _ready(v), _ready(g.to(gates)), _ready(beta.to(gates))),
-                         q.size(-1) ** -.5 if scale is None else float(scale), state, slots)
+    out = cu.delta_step((_ready(q), _ready(k), _ready(v), _ready(g.to(gates)), _ready(beta.to(gates))),
+                        q.size(-1) ** -.5 if scale is None else float(scale), state, slots)
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)  # a graph that has saved the state sees that it has changed
+    return out

@@ -73,3 +73,17 @@ def test_checkpoints_hold_the_masks_key_and_offset():
     assert torch.equal(other.dropout_seed, before) and 'dropout_seed' not in quiet.state_dict()
     holder = torch.nn.ModuleDict(dict(m=make(0.)))
     holder.load_state_dict({f'm.{k}': t for k, t in trained.state_dict().items()})
+
+
+def test_a_refused_step_leaves_the_states_version():
+    """A graph that has saved the state may still be walked."""
+    import dism_b200
+    import pytest
+    import torch
+    dism_b200.install_dropin()
+    import flash_dism
+    q, gates, state = torch.zeros(1, 2, 32, dtype=torch.bfloat16), torch.zeros(1, 2), torch.zeros(1, 2, 32, 32)
+    before = state._version
+    with pytest.raises(RuntimeError, match='invalid device'):
+        flash_dism.gated_delta_step(q, q, q, gates, gates, state)
+    assert state._version == before
