@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_reverse_kernel(DeltaShape
                 *reinterpret_cast<float4*>(ds[n]) = part.lost ? make_float4(NOT_A_NUMBER, NOT_A_NUMBER, NOT_A_NUMBER, NOT_A_NUMBER) : __ldcg(from + n * 32);
         }
         // the gradient behind an earlier segment: dS <- M^T dS + B over the segments behind it, M and dS as pairs as in the forward.  The last one's B already has dfinal.
-        if (!LOCAL && !SHARES)
+        if constexpr (!LOCAL && !SHARES && D >= 64 && WARPS == 4)
             for (int later = behind; later > 0; --later) {
                 const int64_t place = (shape.segments.place(slot) + later) * shape.heads + head;  // of M; B lies one before
                 const float4* end = reinterpret_cast<const float4*>(ends + (place - shape.heads) * D * dv) + column / 16 * (D / 8) * 32 + lane;
@@ -674,10 +674,9 @@ template <int D>
 cudaError_t launch_width(const DeltaShape& shape, const DeltaGradients& x, const DeltaSaved& saved, cudaStream_t stream) {
     cudaError_t status = shape.dv % 64 == 0 ? launch_reverse<D, 4>(shape, x, saved, stream) : launch_reverse<D, 2>(shape, x, saved, stream);
     if (status || shape.layout.slots() == 0) return status;
-    if (D >= 64 && shape.dv >= 64) return launch_delta_gradient_tensor(shape, x, saved, stream);
     if (shape.dv == 32) return launch_gradient<D, 32>(shape, x, saved, stream);
-    if (shape.dv == 64) return launch_gradient<D, 64>(shape, x, saved, stream);
-    return launch_gradient<D, 128>(shape, x, saved, stream);
+    if constexpr (D >= 64) return launch_delta_gradient_tensor(shape, x, saved, stream);
+    else return shape.dv == 64 ? launch_gradient<D, 64>(shape, x, saved, stream) : launch_gradient<D, 128>(shape, x, saved, stream);
 }
 }  // namespace
 

@@ -38,7 +38,6 @@ constexpr int CHUNK = 64;
 // Per chunk and head: e^G, b, e^{G_63 - G}, the product of the last two, and G as a pair of floats.
 constexpr int ROW_DECAY = 0, ROW_BETA = CHUNK, ROW_TAIL = 2 * CHUNK, ROW_WRITE = 3 * CHUNK, ROW_HIGH = 4 * CHUNK, ROW_LOW = 5 * CHUNK, ROW_VALUES = 6 * CHUNK;
 constexpr int MATRIX = 10 * 256;           // elements of T and P of one chunk and head: the 16 x 16 tiles up to the diagonal
-constexpr float LOG2E = 1.4426950408889634f;
 #define NOT_A_NUMBER __int_as_float(0x7fc00000)
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) delta_chain_kernel(DeltaShape s
         // The state at a later segment's start: S <- M S + B over the segments before it.  M and S are pairs here whatever is wanted at the end: a
         // rounding at a join stays in the state, and with slow decays and weak writes (M close to one) single bf16 left 1.1 to 2.2 % of the output's norm
         // after 32 joins.
-        if (!LOCAL && !SHARES)
+        if constexpr (!LOCAL && !SHARES && D >= 64 && WARPS == 4)
             for (int before = 0; before < number; ++before) {
                 const int64_t place = (shape.segments.place(slot) - number + before) * shape.heads + head;
                 load_block<2 * D * D, THREADS>(base, reinterpret_cast<const char*>(shape.segments.m + place * D * D), thread);

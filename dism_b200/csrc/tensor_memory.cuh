@@ -78,7 +78,6 @@ __device__ __forceinline__ void tm_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tm_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tm_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tm_address(bar)) : "memory");
 }
@@ -94,10 +93,6 @@ __device__ __forceinline__ void tm_load16(float (&v)[16], uint32_t at) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
                    "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]) : "r"(at) : "memory");
-}
-__device__ __forceinline__ void tm_store8(uint32_t at, const uint32_t (&v)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 
 // Descriptors of swizzled tiles; `across` is the distance in bytes between blocks of 64 of the index that is not contracted (MN-major).
@@ -116,11 +111,6 @@ __host__ __device__ constexpr uint32_t tm_instruction(int columns, bool a_across
 __device__ __forceinline__ void tm_mma_shared(uint32_t accumulator, uint64_t a, uint64_t b, uint32_t instruction, bool accumulate) {
     asm volatile("{.reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}"
                  ::"r"(accumulator), "l"(a), "l"(b), "r"(instruction), "r"(uint32_t(accumulate)) : "memory");
-}
-// The left operand in tensor memory: lane = row, a column holds two neighbouring bf16 of the contraction.
-__device__ __forceinline__ void tm_mma(uint32_t accumulator, uint32_t a, uint64_t b, uint32_t instruction, bool accumulate) {
-    asm volatile("{.reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}"
-                 ::"r"(accumulator), "r"(a), "l"(b), "r"(instruction), "r"(uint32_t(accumulate)) : "memory");
 }
 
 }  // namespace dism
