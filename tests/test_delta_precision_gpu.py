@@ -22,15 +22,15 @@ def flash():
     return flash_dism
 
 
-def check(flash, x, starts=None, states=False, form=chunked.sequences):
-    """x: operands on the host."""
+def check(flash, x, starts=None, states=False, out_bound=OUT, grad_bound=GRAD, decay_terms=None):
+    """x: operands on the host.  decay_terms: what the error of dg is measured by, from the exact gradients, instead of its norm."""
     g = torch.Generator().manual_seed(1)
     dout = torch.randn(x[2].shape, generator=g).bfloat16().cuda()
     shape = (x[2].shape[0] if starts is None else len(starts) - 1, x[2].shape[2], x[0].shape[3], x[2].shape[3])
     initial, dfinal = (.3 * torch.randn(shape, generator=g).cuda() for _ in range(2)) if states else (None, None)
     more = [initial] if states else []
     exact = [t.cuda().double().requires_grad_() for t in x + more]
-    want, want_state = form(*exact[:5], x[0].shape[-1] ** -.5, exact[5] if states else None, starts)
+    want, want_state = chunked.sequences(*exact[:5], x[0].shape[-1] ** -.5, exact[5] if states else None, starts)
     want_grads = torch.autograd.grad([want, want_state] if states else want, exact, [dout.double(), dfinal.double()] if states else dout.double())
     leaves = [t.cuda().requires_grad_() for t in x + more]
     cu = None if starts is None else torch.tensor(starts, dtype=torch.int32, device='cuda')
@@ -40,10 +40,14 @@ def check(flash, x, starts=None, states=False, form=chunked.sequences):
     errors = dict(out=chunked.norms(out, want, 2))
     for name, got, expected in zip(('q', 'k', 'v', 'g', 'beta', 'initial'), grads, want_grads):
         errors['d' + name] = chunked.norms(got, expected, 1 if name == 'initial' else 2)
+    bounds = dict(out=out_bound, state=STATE)
     if states:
         errors['state'] = chunked.norms(final, want_state, 1)
+    if decay_terms:
+        errors['dg'] = ((grads[3].double() - want_grads[3]).norm(dim=1) / decay_terms(exact, want_grads).norm(dim=1)).max().item()
+        bounds['dg'] = chunked.ROUNDING
     print({name: f'{e:.2e}' for name, e in errors.items()})
-    assert all(e <= dict(out=OUT, state=STATE).get(name, GRAD) for name, e in errors.items()), errors
+    assert all(e <= bounds.get(name, grad_bound) for name, e in errors.items()), errors
 
 
 @pytest.mark.parametrize('n,d,dv', [(16384, 64, 64), (16384, 128, 128), (4099, 128, 64)])
@@ -82,3 +86,66 @@ def test_a_pack_seen_in_inference_mode_trains_afterwards(flash):
     out = flash.gated_delta_rule(*leaves, cu_seqlens=starts)
     assert torch.equal(out, quiet)
     assert all(torch.isfinite(t).all() for t in torch.autograd.grad(out, leaves, torch.ones_like(out)))
+
+
+@pytest.mark.parametrize('key_heads,heads', [(2, 2), (1, 3)])
+@pytest.mark.parametrize('d,dv', [(32, 32), (32, 128), (64, 64), (64, 128), (128, 32), (128, 64), (128, 128)])
+def test_training_at_every_width(flash, d, dv, key_heads, heads):
+    """No state asked for, key heads shared and not."""
+    check(flash, reference.operands(d + dv, 2, 333, key_heads, heads, d, dv, gates=torch.float32 if heads == 3 else torch.bfloat16))
+
+
+@pytest.mark.parametrize('decay', [1e-4, .02, .5, 4.])
+def test_training_at_any_decay(flash, decay):
+    check(flash, reference.operands(7, 1, 700, 1, 2, 128, 128, decay=decay))
+
+
+@pytest.mark.parametrize('d,dv,key_heads', [(64, 64, 1), (128, 128, 2), (128, 64, 1), (64, 128, 2)])
+def test_training_on_cut_chains(flash, d, dv, key_heads):
+    check(flash, reference.operands(d, 1, 3001, key_heads, 2, d, dv, decay=.02))
+
+
+@pytest.mark.parametrize('d,dv,starts', [(128, 128, [0, 1, 2, 66, 130, 130, 257]), (64, 64, [0, 0, 64, 128, 200]), (32, 64, [4, 90, 300]), (128, 128, [0, 600, 2400])])
+def test_training_on_packs(flash, d, dv, starts):
+    check(flash, reference.operands(len(starts), 1, starts[-1], 2, 4, d, dv, decay=.1), starts=starts)
+
+
+@pytest.mark.parametrize('d,dv', [(64, 64), (128, 128)])
+@pytest.mark.parametrize('states', [False, True])
+def test_shares_against_64_bits(flash, d, dv, states):
+    """A few more chains than places, long enough to be walked in equal shares."""
+    room = 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    check(flash, reference.operands(d, (room + 8) * 64 // (4 * dv), 577, 2, 4, d, dv, decay=.02), states=states)
+
+
+def test_repeated_keys_in_training(flash):
+    """One key for a whole chunk and write strengths of one, the worst case of the chunk's inverse: its rows cancel, so roundings are
+    not small beside what is left of them, and each is counted in full (2^-8) and added.
+
+    dg is what is left of larger terms: a factor on every state from position t on can be moved to q from t on and, inverted, to v, so dg_t is the sum
+    over j >= t of q_j.dq_j - v_j.dv_j; and the kernels reach v_j.dv_j through k_j.dk_j, by adding beta_j dbeta_j and taking it away.  Each of these
+    comes out of products of bf16 operands, so even with nothing else rounded one rounding of the terms, in quadrature over a chunk, is left
+    in dg.  Here the terms are a hundred times dg (norms 2.4e2 and 2.4 for the first head): dg is held to one rounding of them."""
+    x = reference.operands(11, 1, 200, 2, 2, 128, 64, decay=.02)
+    x[1][:, 20:100] = x[1][:, 20:21]
+    x[0][:, 50:] = x[1][:, 50:]
+    x[4].fill_(1.)
+
+    def terms(exact, grads):
+        q, k, v, g, beta = exact
+        each = (q * grads[0]).sum(-1).square() + (v * grads[2]).sum(-1).square() + 2 * (beta * grads[4]).square()
+        chunks = torch.nn.functional.pad(each, (0, 0, 0, -each.shape[1] % 64)).unflatten(1, (-1, 64))
+        return chunks.flip(2).cumsum(2).flip(2).flatten(1, 2)[:, :each.shape[1]].sqrt()
+    check(flash, x, out_bound=6 * 2 ** -8, grad_bound=12 * 2 ** -8, decay_terms=terms)
+
+
+def test_only_the_last_state_is_asked_for(flash):
+    """A loss of the final state alone: no gradient reaches the output."""
+    x = reference.operands(12, 2, 150, 1, 2, 64, 64)
+    exact = [t.cuda().double().requires_grad_() for t in x]
+    weight = torch.randn(2, 2, 64, 64, generator=torch.Generator().manual_seed(2)).cuda()
+    want = torch.autograd.grad((chunked.sequences(*exact, 64 ** -.5)[1] * weight.double()).sum(), exact[1:])
+    leaves = [t.cuda().requires_grad_() for t in x]
+    got = torch.autograd.grad((flash.gated_delta_rule(*leaves, output_final_state=True)[1] * weight).sum(), leaves)
+    assert not got[0].count_nonzero()
+    assert all(chunked.norms(a, b, 2) <= GRAD for a, b in zip(got[1:], want))
