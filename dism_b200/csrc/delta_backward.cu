@@ -3,7 +3,7 @@
 //     dS0 = e^{G_63} dS1 + (scale e^G Q)^T dO - (e^G K)^T dY.
 // delta_reverse_kernel walks the chunks from the last to the first with dS, transposed, in its accumulators (a warp owns 16
 // columns, as in the forward chain), writes dV, keeps every dS1 and the part of db that needs dU.
-// As the forward chain it is bound by latency: 166 us at 16 x 2048 positions, 10 heads of 128 (in shares); segments of 2 x 8192, 16 heads of 64: 39 + 64.
+// As the forward chain it is bound by latency: 167 us at 16 x 2048 positions, 10 heads of 128 (in shares); segments of 2 x 8192, 16 heads of 64: 39 + 68.
 // delta_gradient_kernel then takes all chunks at once (here for D or DV of 32; delta_gradient.cu has the others).  With Z1 = dO X^T and Z2 = dY X^T,
 //     dP~ = scale E b_s Z1 (s <= t),   dL~ = -E b_s Z2 (s < t),
 //     dQ = scale e^G dO S0^T + dP~ K,

@@ -12,7 +12,7 @@
 // 64, uncut: 279 / 209; prompt of 16384, 16 heads of 128, uncut: 850 / 762; 500, 4 heads: 38 to 45 / 27.
 // What bounds it: with four warps a CTA and two CTAs an SM, latency of dependent instructions (one or two warps to a scheduler; the main
 // stall is the fixed latency of an instruction, with one CTA an SM the tensor pipe is 47 % busy).  16 x 2048 positions, 10 heads of 128
-// (320 chains for 296 places): 177 us in shares, 250 as 320 CTAs; as segments 2 x 8192, 16 heads of 64: 62 + 66 us.
+// (320 chains for 296 places): 175 us in shares, 250 as 320 CTAs; as segments 2 x 8192, 16 heads of 64: 62 + 76 us (66 with joins of single operands).
 //
 // What is rounded: products take bf16, so every operand that is not one already is rounded, once, or kept as a pair (value and
 // remainder, 16 bits) for a second product.  Y and what is added to the state are pairs always: these roundings would reach every
@@ -391,8 +391,9 @@ cudaError_t by_width(const DeltaShape& shape, const __nv_bfloat16* q, const __nv
 }  // namespace
 
 // A segment costs two CTA walks forward (one of them for B and M, without outputs) and two backward, so cutting pays when the walks
-// get at least four times shorter; with segments of equal length for two CTAs per SM (what the chains' registers and shared memory
-// allow), but no shorter than eight chunks, below which putting the starts together costs what it saves.  Measured, forward and
+// get at least four times shorter; the chunks are divided by the places of two CTAs per SM (what the chains' registers and shared memory
+// allow), but a segment has no fewer than eight, below which putting the starts together costs what it saves.  Every sequence rounds up to whole segments, so
+// the second launch may have a few more CTAs than places: 320 on 296 at the first two shapes below.  Measured, forward and
 // backward chain with single operands, uncut / for one / for two CTAs per SM (us): 2 x 8192, 16 heads of 64: 426 / 281 / 211; prompt of 16384, 16 heads of
 // 128: 761 / 523 / 439; pack of 7019, 8 heads: 166 / 152 / 120.  4 x 2048, 10 heads of 128 (32 chunks to 9): 204 / - / 212.
 int delta_segment_length(const DeltaLayout& layout, int heads, int d, int dv) {

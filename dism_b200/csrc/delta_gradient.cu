@@ -16,8 +16,8 @@
 // (boxes of tensor maps; where a chunk ends inside a tile the rows behind it, another document's, are made zeros), one puts the 64 values each of dg and db together.  The
 // end of Z, QK, U1, V1 and the trace frees every tile but Q, K (of which there are two) and the pairs, and the next item's loads run
 // behind the rest of this one.
-// 212 us for 5120 items of D = DV = 128 (16 x 2048 positions, 10 heads): 180 KB in and out an item, its intermediates
-// included, 4.4 TB/s or 0.69 of the measured copy rate; 121 us for 2 x 8192, 16 heads of 64.  With a tensor pipe at 22 % and DRAM at 39 % (a
+// 203 us for 5120 items of D = DV = 128 (16 x 2048 positions, 10 heads): 180 KB in and out an item, its intermediates
+// included, 4.6 TB/s or 0.72 of the measured copy rate; 113 us for 2 x 8192, 16 heads of 64.  With a tensor pipe at 22 % and DRAM at 39 % (a
 // quarter of that size) it is bound by the latency of an item's phases.  Steps on the way, same shape: mma.sync tiles 511 us, one CTA an item on tcgen05 433, the next item's loads
 // behind the present one 281, loops rolled for the instruction cache 262, whole-line stores 249, boxes and roles 212.
 #include "delta_common.cuh"

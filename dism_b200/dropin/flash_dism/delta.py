@@ -122,7 +122,7 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, output
     [B,N,H,DV]; with output_final_state=True also the FP32 state [sequences,H,D,DV] after each sequence's last position.
 
     H is a multiple of HK (value head h reads key head h // (H // HK)), D and DV in {32,64,128}, N any length.  Keys are meant to
-    have length one at most; the caller normalises.  scale defaults to D ** -0.5.  g = -inf clears the state.  A pack is one
+    have length one at most; the caller normalises.  scale defaults to D ** -0.5.  g = -inf clears a finite state.  A pack is one
     batch row with either `layout` (a VarlenLayout) or `cu_seqlens`, int32 [documents+1]; documents may have any length, zero
     included.  On the CPU cu_seqlens is validated (and like a layout uploaded once, which has to happen before a
     capture); on the GPU it is read by the kernels only (so a captured graph can follow new

@@ -165,13 +165,13 @@ int dism_longest_match(const int32_t *streams, int batch, int n, int32_t *end, i
  * dism_v3/python/flash_dism/hybrid_gdn.py, pure_gdn.py).  Per value head, with a state S [D,DV] in FP32:
  *   S_t = exp(g_t) S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - exp(g_t) S_{t-1}^T k_t),  o_t = scale S_t^T q_t.
  * q, k bf16 [B,N,HK,D]; v, out bf16 [B,N,H,DV], H a multiple of HK (value head h reads key head h / (H/HK));
- * g (natural-log decay; minus infinity clears the state) and beta [B,N,H], float or (gates_bf16) bf16; D, DV in {32,64,128};
+ * g (natural-log decay; minus infinity clears a finite state) and beta [B,N,H], float or (gates_bf16) bf16; D, DV in {32,64,128};
  * any N.  States float [sequences,H,D,DV].  cu_seqlens NULL: `sequences` rows of n positions.  Packed: one row of n positions,
  * cu_seqlens device int32 [sequences+1]; document i is [cu[i], cu[i+1]), any length, empty ones included.  The library cannot
  * read the table on the host: entries are clamped to [0, n], so no table reaches outside the tensors, but the results are
  * defined only for ascending ones; rows before the first and behind the last document come out as zeros.  initial_state NULL: zeros; final_state NULL: not wanted.
- * The chain of chunks takes V - e^G K S and what it adds to the state as pairs of bf16 (16 bits); with a final state the state and the
- * chunk's inverse too, without one those are single bf16.
+ * The chain of chunks takes V - e^G K S and what it adds to the state as pairs of bf16 (16 bits), and so the state where the
+ * segments of a long chain are joined; with a final state also the state in the products and the chunk's inverse, without one those are single bf16.
  * `saved`: dism_delta_saved bytes, 256-byte aligned; dead after the call unless `backward` is set: then dism_delta_backward
  * of the same call takes it (a size computed with final_state serves both).  The sizes are those of the current device. */
 size_t dism_delta_saved(int packed, int sequences, int n, int heads, int d, int dv, int final_state, int backward);
