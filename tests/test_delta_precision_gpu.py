@@ -149,3 +149,33 @@ def test_only_the_last_state_is_asked_for(flash):
     got = torch.autograd.grad((flash.gated_delta_rule(*leaves, output_final_state=True)[1] * weight).sum(), leaves)
     assert not got[0].count_nonzero()
     assert all(chunked.norms(a, b, 2) <= GRAD for a, b in zip(got[1:], want))
+
+
+@pytest.mark.parametrize('b,n,heads', [(75, 577, 4), (1, 4100, 2)])
+def test_captured_training_step(flash, b, n, heads):
+    """Walked in shares and cut into segments: replays follow new inputs, two graphs in turn do not disturb one another."""
+    sets = [[t.cuda() for t in reference.operands(seed, b, n, 1, heads, 64, 64, decay=.02)] for seed in (1, 2)]
+    dout = torch.randn_like(sets[0][2])
+
+    def step(leaves):
+        out = flash.gated_delta_rule(*leaves)
+        return [out, *torch.autograd.grad(out, leaves, dout)]
+    wanted = [step([t.clone().requires_grad_() for t in x]) for x in sets]
+    wanted = [[t.detach() for t in w] for w in wanted]
+    graphs = []
+    for x in sets:
+        held = [t.clone().requires_grad_() for t in x]
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            got = step(held)
+        graphs.append((graph, held, got))
+    for turn in range(4):
+        graph, held, got = graphs[turn % 2]
+        other = (turn // 2 + turn) % 2
+        with torch.no_grad():
+            for t, new in zip(held, sets[other]):
+                t.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(got, wanted[other]))
